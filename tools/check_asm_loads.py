@@ -228,7 +228,7 @@ def main():
     with tempfile.TemporaryDirectory() as d:
         out = os.path.join(d, "k.s")
         subprocess.run([HIPCC, "-O3", "-std=c++17", "--offload-arch=gfx950", "--cuda-device-only",
-                        "-S", "-o", out, SRC], check=True, capture_output=True)
+                        "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-S", "-o", out, SRC], check=True, capture_output=True)
         asm = open(out).read()
     found, n = 0, 0
     for name, body in kernels(asm):
