@@ -1,0 +1,1289 @@
+// Differential attention over the in-neighbours of every node, and the learned relative position
+// bias its logits can carry:
+//   x_m[e,h] = scale q[i,h,m] . k[j,h,m] + bias[bucket[e],h]        (e = j -> i, m = 1, 2)
+//   out[i,h] = sum_e (p_1 - lam_h p_2) v[j,h],   p_m = softmax of x_m over i's edges
+// Backward, with w = p_1 - lam p_2, dw_e = go[i] . v[j], D_m = sum_e p_m dw:
+//   dx_1 = p_1 (dw - D_1),  dx_2 = -lam p_2 (dw - D_2)
+//   gq_m[i] = scale sum_e dx_m k_m[j];  gk_m[j] = scale sum_e dx_m q_m[i];  gv[j] = sum_e w go[i]
+//   glam_h = -sum_i D_2;  gbias[b,h] = sum over b's edges of dx_1 + dx_2
+//
+// Bound by the gathers: every edge reads (2d + dv) elements of its source's (or destination's) row
+// per head, from L2 as long as one head's rows of the nodes in flight fit there. So a work item is
+// (row, head), items run in chunks of kChunk rows one head after the other, and whole (chunk, head)
+// units go to one XCD. The products are sparse (a row's neighbours are shared with no other row),
+// so they run on the vector units: packed dot products for the 16-bit types, and sums in fp32.
+//
+// G lanes hold one edge: lane c of them the c-th 8-element chunk of both maps' keys and the chunks
+// c (and c + G) of the values, so a logit is one exchange over G lanes and nothing else crosses
+// lanes. 64 / G edges are in flight per wave ("slots"), `rows_per_wave` rows share the wave where
+// their degree would leave slots idle. Each slot keeps its own running maxima and sums over its
+// edges (one pass over the data), joined when the row ends. Rows of more than hub_edges edges, and
+// the few rows of a serving call, are cut into pieces with partial results, joined in piece order.
+// The backward is three gathers: dw and D over the values (A), gq over the keys (B, which also
+// leaves {scale dx_1, scale dx_2, w} of each edge), gk and gv over the queries and go by the
+// transposed CSR (C). Every sum has a fixed order.
+#include "dtypes.h"
+
+namespace gatx {
+namespace {
+
+constexpr int kChunk = 2048;       // rows of a (chunk, head) unit
+constexpr int kMaxD = 256, kMaxDv = 512, kMaxBuckets = 256;
+constexpr float kInf = __builtin_huge_valf();
+constexpr float kLog2e = 1.44269504088896341f;
+
+// ------------------------------------------------------------------ 8 elements of a row
+template <typename T>
+struct Raw {
+  uint4 v;
+};
+template <>
+struct Raw<float> {
+  float4 a, b;
+};
+template <typename T>
+__device__ inline Raw<T> load8(const T* p) {
+  Raw<T> r;
+  r.v = *reinterpret_cast<const uint4*>(p);
+  return r;
+}
+template <>
+__device__ inline Raw<float> load8<float>(const float* p) {
+  Raw<float> r;
+  r.a = *reinterpret_cast<const float4*>(p);
+  r.b = *reinterpret_cast<const float4*>(p + 4);
+  return r;
+}
+template <typename T>
+__device__ inline Raw<T> zero8() {
+  Raw<T> r;
+  r.v = make_uint4(0, 0, 0, 0);
+  return r;
+}
+template <>
+__device__ inline Raw<float> zero8<float>() {
+  Raw<float> r;
+  r.a = r.b = make_float4(0, 0, 0, 0);
+  return r;
+}
+template <typename T>
+__device__ inline Raw<T> keep8(bool keep, Raw<T> x) {
+  x.v.x = keep ? x.v.x : 0u;
+  x.v.y = keep ? x.v.y : 0u;
+  x.v.z = keep ? x.v.z : 0u;
+  x.v.w = keep ? x.v.w : 0u;
+  return x;
+}
+__device__ inline Raw<float> keep8(bool keep, Raw<float> x) {
+  x.a = make_float4(keep ? x.a.x : 0.f, keep ? x.a.y : 0.f, keep ? x.a.z : 0.f, keep ? x.a.w : 0.f);
+  x.b = make_float4(keep ? x.b.x : 0.f, keep ? x.b.y : 0.f, keep ? x.b.z : 0.f, keep ? x.b.w : 0.f);
+  return x;
+}
+
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+__device__ inline float dot2(__bf16, uint32_t a, uint32_t b, float c) {
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, a),
+                                         __builtin_bit_cast(bf16x2, b), c, false);
+}
+__device__ inline float dot2(_Float16, uint32_t a, uint32_t b, float c) {
+  return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, a), __builtin_bit_cast(f16x2, b), c,
+                                false);
+}
+template <typename T>
+__device__ inline float dot8(const Raw<T>& a, const Raw<T>& b, float c) {
+  c = dot2(T(), a.v.x, b.v.x, c);
+  c = dot2(T(), a.v.y, b.v.y, c);
+  c = dot2(T(), a.v.z, b.v.z, c);
+  return dot2(T(), a.v.w, b.v.w, c);
+}
+__device__ inline float dot8(const Raw<float>& a, const Raw<float>& b, float c) {
+  c = fmaf(a.a.x, b.a.x, c);
+  c = fmaf(a.a.y, b.a.y, c);
+  c = fmaf(a.a.z, b.a.z, c);
+  c = fmaf(a.a.w, b.a.w, c);
+  c = fmaf(a.b.x, b.b.x, c);
+  c = fmaf(a.b.y, b.b.y, c);
+  c = fmaf(a.b.z, b.b.z, c);
+  return fmaf(a.b.w, b.b.w, c);
+}
+
+__device__ inline float2 unpack2(__bf16, uint32_t x) {
+  return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
+}
+__device__ inline float2 unpack2(_Float16, uint32_t x) {
+  const f16x2 h = __builtin_bit_cast(f16x2, x);
+  return make_float2((float)h.x, (float)h.y);
+}
+template <typename T>
+__device__ inline void unpack8(const Raw<T>& x, float (&f)[8]) {
+  const uint32_t w[4] = {x.v.x, x.v.y, x.v.z, x.v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 p = unpack2(T(), w[i]);
+    f[2 * i] = p.x;
+    f[2 * i + 1] = p.y;
+  }
+}
+__device__ inline void unpack8(const Raw<float>& x, float (&f)[8]) {
+  f[0] = x.a.x; f[1] = x.a.y; f[2] = x.a.z; f[3] = x.a.w;
+  f[4] = x.b.x; f[5] = x.b.y; f[6] = x.b.z; f[7] = x.b.w;
+}
+__device__ inline void axpy8(float p, const float (&x)[8], float (&acc)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) acc[i] = fmaf(p, x[i], acc[i]);
+}
+template <typename T>
+__device__ inline void axpy8(float p, const Raw<T>& x, float (&acc)[8]) {
+  float f[8];
+  unpack8(x, f);
+  axpy8(p, f, acc);
+}
+// Columns [at, at + 8) of a packed row of `width` elements.
+template <typename T>
+__device__ inline void store8(T* row, int at, int width, bool whole, const float (&x)[8]) {
+  if (whole) {
+    if (at >= width) return;
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<float4*>(row + at) = make_float4(x[0], x[1], x[2], x[3]);
+      *reinterpret_cast<float4*>(row + at + 4) = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+      store_f32<T, 8>(row + at, x);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (at + i < width) row[at + i] = (T)x[i];
+  }
+}
+
+// ------------------------------------------------------------------ lanes of a wave
+// Sums over the G lanes of an edge.
+template <int G>
+__device__ inline float edge_sum(float v) {
+  return group_sum<G>(v);
+}
+// Sum over the slots of a row (lanes l, l + G, ... of its GS), in every lane. Rotations inside 16
+// lanes, swaps beyond; GS >= 16.
+template <int G>
+__device__ inline float slots_sum(float v, int gs) {
+  if (G <= 8) v += dpp<0x128>(v);   // row_ror:8
+  if (G <= 4) v += dpp<0x124>(v);
+  if (G <= 2) v += dpp<0x122>(v);
+  if (G <= 1) v += dpp<0x121>(v);
+  if (G <= 16 && gs >= 32) {
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+  if (gs >= 64) {
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+  return v;
+}
+template <int G>
+__device__ inline float slots_max(float v, int gs) {
+  for (int d = G; d < gs; d <<= 1) v = fmaxf(v, __shfl_xor(v, d));
+  return v;
+}
+__device__ inline int wave_max(int v) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) v = max(v, __shfl_xor(v, d));
+  return __builtin_amdgcn_readfirstlane(v);
+}
+__device__ inline float exp_(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
+
+// ------------------------------------------------------------------ work items
+// Which (row, head, edges) a group of `gs` lanes has.
+struct Work {
+  // plain rows: units of `chunk` rows of one head, dealt to the XCDs in turn
+  int64_t rows;
+  int heads, chunk, gs;
+  int64_t units;            // ceil(rows / chunk) * heads
+  int blocks_per_unit;
+  const int32_t* rowptr;
+  // pieces: of hub rows (hubs != NULL: the plan's entries), or of the rows of a serving call
+  // (nodes != NULL: `pieces` of each)
+  int hub_edges;
+  const int32_t *hubs, *hub_count;
+  int64_t hub_bound, hub_blocks;   // blocks [0, hub_blocks) have the pieces
+  const int64_t* nodes;
+  int pieces;
+  int64_t num_nodes;
+};
+struct Item {
+  int64_t row;    // of the outputs and of q; < 0: none
+  int64_t slot;   // of the partial results; < 0: this item is the whole row
+  int head, beg, end;
+  bool bad;       // a node id that does not exist
+};
+__device__ inline Item find_item(const Work& w) {
+  const int per_block = 256 / w.gs, grp = (int)threadIdx.x / w.gs;
+  Item it = {-1, -1, 0, 0, 0, false};
+  if (w.nodes) {
+    const int64_t i = (int64_t)blockIdx.x * per_block + grp;
+    if (i >= w.rows * w.heads * w.pieces) return it;
+    const int64_t rh = i / w.pieces;
+    const int piece = (int)(i - rh * w.pieces);
+    it.row = rh / w.heads;
+    it.head = (int)(rh - it.row * w.heads);
+    it.slot = w.pieces > 1 ? it.row * w.pieces + piece : -1;
+    const int64_t n = w.nodes[it.row];
+    it.bad = n < 0 || n >= w.num_nodes;
+    if (it.bad) return it;
+    const int b = w.rowptr[n], e = w.rowptr[n + 1];
+    const int len = (int)(((int64_t)e - b + w.pieces - 1) / w.pieces);
+    it.beg = (int)min((int64_t)e, b + (int64_t)piece * len);
+    it.end = (int)min((int64_t)e, (int64_t)it.beg + len);
+    return it;
+  }
+  if (blockIdx.x < w.hub_blocks) {
+    const int64_t i = (int64_t)blockIdx.x * per_block + grp;
+    const int64_t pc = i / w.heads;
+    if (pc >= w.hub_bound || pc >= *w.hub_count) return it;
+    const int32_t* hp = w.hubs + 4 * pc;
+    it.row = hp[0];
+    it.head = (int)(i - pc * w.heads);
+    it.slot = pc;
+    it.beg = w.rowptr[it.row] + hp[1] * w.hub_edges;
+    it.end = (int)min((int64_t)w.rowptr[it.row + 1], (int64_t)it.beg + w.hub_edges);
+    return it;
+  }
+  const int64_t b = blockIdx.x - w.hub_blocks;
+  const int64_t j = b / 8;
+  const int64_t unit = j / w.blocks_per_unit * 8 + b % 8;
+  if (unit >= w.units) return it;
+  const int64_t ck = unit / w.heads;
+  const int64_t in = (j % w.blocks_per_unit) * per_block + grp;
+  const int64_t row = ck * w.chunk + in;
+  if (in >= w.chunk || row >= w.rows) return it;
+  it.head = (int)(unit - ck * w.heads);
+  it.beg = w.rowptr[row];
+  it.end = w.rowptr[row + 1];
+  if (w.hub_edges > 0 && it.end - it.beg > w.hub_edges) return it;   // in pieces, above
+  it.row = row;
+  return it;
+}
+
+struct AttnArgs {
+  Work w;
+  const void *q, *k, *v, *go;
+  int64_t ldq, ldk, ldv, ldgo;
+  int d, dv, dp, dvp;
+  const int32_t* col;        // (C: scol)
+  const int32_t* seid;       // C
+  int64_t E;
+  float scale;
+  const float *lam, *bias;
+  const uint8_t* bucket;
+  float2* S;                 // [H][E] logits
+  float4* stat;              // [H][rows] {max1, 1/sum1, max2, 1/sum2}
+  void* out;
+  float* part;               // [slot][H][part_width]
+  int part_width;
+  // backward
+  float* dw;                 // [H][E]
+  float2* D;                 // [H][rows]
+  float4* rec;               // [H][E] {scale dx1, scale dx2, w, dx1 + dx2}
+  void *gq, *gk, *gv;
+};
+
+// One row's state over a slot's edges: both maps' running maximum and sum.
+template <int NV>
+struct Acc {
+  float m1 = -kInf, m2 = -kInf, l1 = 0.f, l2 = 0.f;
+  float a1[NV][8] = {}, a2[NV][8] = {};
+};
+__device__ inline float finite_max(float m) { return m == -kInf ? 0.f : m; }
+
+// U edges of a slot. CHECK: some lane of the wave has an edge that is past its row's end or shut;
+// what such an edge points at is not let into the sums.
+template <typename T, int G, int NV, int U, bool BIAS, bool CHECK>
+__device__ inline void forward_step(const Raw<T> (&k1)[U], const Raw<T> (&k2)[U],
+                                    const Raw<T> (&v)[U][NV], const Raw<T>& q1, const Raw<T>& q2,
+                                    const float (&b)[U], const bool (&open)[U], float scale,
+                                    Acc<NV>& acc, float2 (&x)[U]) {
+  float n1 = acc.m1, n2 = acc.m2;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    x[u].x = edge_sum<G>(dot8(q1, k1[u], 0.f)) * scale;
+    x[u].y = edge_sum<G>(dot8(q2, k2[u], 0.f)) * scale;
+    if (BIAS) {
+      x[u].x += b[u];
+      x[u].y += b[u];
+    }
+    if (CHECK) {
+      x[u].x = open[u] ? x[u].x : -kInf;
+      x[u].y = open[u] ? x[u].y : -kInf;
+    }
+    n1 = fmaxf(n1, x[u].x);
+    n2 = fmaxf(n2, x[u].y);
+  }
+  const float r1 = finite_max(n1), r2 = finite_max(n2);
+  const float c1 = exp_(acc.m1 - r1), c2 = exp_(acc.m2 - r2);
+  acc.m1 = n1;
+  acc.m2 = n2;
+  acc.l1 *= c1;
+  acc.l2 *= c2;
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      acc.a1[j][i] *= c1;
+      acc.a2[j][i] *= c2;
+    }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const float p1 = exp_(x[u].x - r1), p2 = exp_(x[u].y - r2);
+    acc.l1 += p1;
+    acc.l2 += p2;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      float f[8];
+      unpack8(CHECK ? keep8(open[u], v[u][j]) : v[u][j], f);
+      axpy8(p1, f, acc.a1[j]);
+      axpy8(p2, f, acc.a2[j]);
+    }
+  }
+}
+
+// Edges in flight per slot
+template <typename T>
+struct Unroll {
+  static constexpr int kForward = sizeof(T) == 4 ? 2 : 4;
+};
+
+template <typename T, int G, int NV, bool BIAS, bool SAVE>
+__global__ void __launch_bounds__(256) diff_forward_kernel(AttnArgs a) {
+  constexpr int U = Unroll<T>::kForward;
+  const Item it = find_item(a.w);
+  const int gs = a.w.gs, lane = threadIdx.x & (gs - 1);
+  const int c = lane % G, slot = lane / G, slots = gs / G;
+  const int dch = a.dp / 8, vch = a.dvp / 8;
+  const bool has = it.row >= 0;
+  const int64_t row = has ? it.row : 0;
+  Raw<T> q1 = zero8<T>(), q2 = zero8<T>();
+  if (has && c < dch) {
+    const T* q = (const T*)a.q + row * a.ldq + (int64_t)it.head * 2 * a.dp + c * 8;
+    q1 = load8(q);
+    q2 = load8(q + a.dp);
+  }
+  Acc<NV> acc;
+  const T* kb = (const T*)a.k + (int64_t)it.head * 2 * a.dp + c * 8;
+  const T* vb = (const T*)a.v + (int64_t)it.head * a.dvp + c * 8;
+  const int n = has ? it.end - it.beg : 0;
+  const int turns = wave_max((n + slots * U - 1) / (slots * U));
+  for (int t = 0; t < turns; ++t) {
+    Raw<T> k1[U], k2[U], v[U][NV];
+    float b[U];
+    bool open[U], all = true;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int o = (t * U + u) * slots + slot;
+      open[u] = o < n;
+      // past the end: the row's first edge (row 0 where there is none), kept out by CHECK
+      const int e = open[u] ? it.beg + o : it.beg;
+      const int64_t j = n > 0 ? a.col[e] : 0;
+      b[u] = 0.f;
+      if (BIAS && n > 0) {
+        b[u] = a.bias[(int)a.bucket[e] * a.w.heads + it.head];
+        open[u] = open[u] && b[u] != -kInf;
+      }
+      all = all && open[u];
+      k1[u] = k2[u] = zero8<T>();
+      if (c < dch) {
+        k1[u] = load8(kb + j * a.ldk);
+        k2[u] = load8(kb + j * a.ldk + a.dp);
+      }
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        v[u][i] = zero8<T>();
+        if (c + i * G < vch) v[u][i] = load8(vb + j * a.ldv + i * G * 8);
+      }
+    }
+    float2 x[U];
+    if (__all(all))
+      forward_step<T, G, NV, U, BIAS, false>(k1, k2, v, q1, q2, b, open, a.scale, acc, x);
+    else
+      forward_step<T, G, NV, U, BIAS, true>(k1, k2, v, q1, q2, b, open, a.scale, acc, x);
+    if (SAVE && c == 0) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int o = (t * U + u) * slots + slot;
+        if (o < n) a.S[(int64_t)it.head * a.E + it.beg + o] = x[u];
+      }
+    }
+  }
+  // the slots joined
+  const float m1 = slots_max<G>(acc.m1, gs), m2 = slots_max<G>(acc.m2, gs);
+  const float c1 = exp_(acc.m1 - finite_max(m1)), c2 = exp_(acc.m2 - finite_max(m2));
+  const float l1 = slots_sum<G>(acc.l1 * c1, gs), l2 = slots_sum<G>(acc.l2 * c2, gs);
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      acc.a1[j][i] = slots_sum<G>(acc.a1[j][i] * c1, gs);
+      acc.a2[j][i] = slots_sum<G>(acc.a2[j][i] * c2, gs);
+    }
+  if (!has || slot != 0) return;
+  if (it.slot >= 0) {   // a piece: {m1, l1, m2, l2, sums of map 1, of map 2}
+    float* p = a.part + (it.slot * a.w.heads + it.head) * a.part_width;
+    if (c == 0) *(float4*)p = make_float4(m1, it.bad ? __builtin_nanf("") : l1, m2, l2);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      store8(p + 4, (c + j * G) * 8, a.dvp, true, acc.a1[j]);
+      store8(p + 4 + a.dvp, (c + j * G) * 8, a.dvp, true, acc.a2[j]);
+    }
+    return;
+  }
+  const float i1 = l1 == 0.f ? 0.f : 1.f / l1, i2 = l2 == 0.f ? 0.f : 1.f / l2;
+  const float w2 = a.lam[it.head] * i2;
+  if (SAVE && c == 0)
+    a.stat[(int64_t)it.head * a.w.rows + row] =
+        make_float4(finite_max(m1), i1, finite_max(m2), i2);
+  T* out = (T*)a.out + (row * a.w.heads + it.head) * a.dv;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    float o[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      o[i] = acc.a1[j][i] * i1 - acc.a2[j][i] * w2;
+      if (it.bad) o[i] = __builtin_nanf("");
+    }
+    store8(out, (c + j * G) * 8, a.dv, a.dv == a.dvp, o);
+  }
+}
+
+// The pieces of a row joined in order: a workgroup per (row, head), 4 runs of pieces side by side.
+template <typename T>
+__global__ void __launch_bounds__(1024) diff_join_kernel(AttnArgs a) {
+  extern __shared__ __attribute__((aligned(16))) float lds[];   // [4][2 dvp]
+  int64_t row, first;
+  int head, pieces;
+  if (a.w.nodes) {
+    row = blockIdx.x / a.w.heads;
+    head = (int)(blockIdx.x - row * a.w.heads);
+    first = row * a.w.pieces;
+    pieces = a.w.pieces;
+  } else {
+    const int64_t pc = blockIdx.x / a.w.heads;
+    if (pc >= *a.w.hub_count) return;
+    const int32_t* hp = a.w.hubs + 4 * pc;
+    if (hp[1] != 0) return;   // a hub's first entry speaks for it
+    row = hp[0];
+    head = (int)(blockIdx.x - pc * a.w.heads);
+    pieces = hp[2];
+    first = pc;
+  }
+  const int H = a.w.heads;
+  const float* p0 = a.part + (first * H + head) * a.part_width;
+  const int64_t step = (int64_t)H * a.part_width;
+  float m1 = -kInf, m2 = -kInf;
+  for (int i = threadIdx.x & 63; i < pieces; i += 64) {
+    m1 = fmaxf(m1, p0[i * step]);
+    m2 = fmaxf(m2, p0[i * step + 2]);
+  }
+  for (int d = 1; d < 64; d <<= 1) {
+    m1 = fmaxf(m1, __shfl_xor(m1, d));
+    m2 = fmaxf(m2, __shfl_xor(m2, d));
+  }
+  const float r1 = finite_max(m1), r2 = finite_max(m2);
+  float l1 = 0.f, l2 = 0.f;
+  for (int i = threadIdx.x & 63; i < pieces; i += 64) {
+    l1 += p0[i * step + 1] * exp_(p0[i * step] - r1);
+    l2 += p0[i * step + 3] * exp_(p0[i * step + 2] - r2);
+  }
+  l1 = group_sum<64>(l1);
+  l2 = group_sum<64>(l2);
+  const int W = 2 * a.dvp, runs = 4, run = threadIdx.x >> 8, t = threadIdx.x & 255;
+  for (int x = t; x < W; x += 256) {
+    const bool second = x >= a.dvp;
+    const float r = second ? r2 : r1;
+    float s = 0.f;
+#pragma unroll 4
+    for (int i = run; i < pieces; i += runs)
+      s += p0[i * step + 4 + x] * exp_(p0[i * step + (second ? 2 : 0)] - r);
+    lds[run * W + x] = s;
+  }
+  __syncthreads();
+  const float i1 = l1 == 0.f ? 0.f : 1.f / l1, i2 = l2 == 0.f ? 0.f : 1.f / l2;
+  const float w2 = a.lam[head] * i2;
+  T* out = (T*)a.out + (row * H + head) * a.dv;
+  for (int x = threadIdx.x; x < a.dv; x += 1024) {
+    float s1 = 0.f, s2 = 0.f;
+    for (int k = 0; k < runs; ++k) {
+      s1 += lds[k * W + x];
+      s2 += lds[k * W + a.dvp + x];
+    }
+    out[x] = (T)(s1 * i1 - s2 * w2);
+  }
+  if (a.stat && threadIdx.x == 0)
+    a.stat[(int64_t)head * a.w.rows + row] = make_float4(r1, i1, r2, i2);
+}
+
+// ------------------------------------------------------------------ backward
+// Both maps' weights of an edge from its logits; a shut or -inf logit has weight 0 whatever the
+// statistics hold.
+__device__ inline float2 weights(float2 x, const float4& st) {
+  return make_float2(x.x == -kInf ? 0.f : exp_(x.x - st.x) * st.y,
+                     x.y == -kInf ? 0.f : exp_(x.y - st.z) * st.w);
+}
+
+// A: dw = go . v of every edge, D_1 and D_2 of every row.
+template <typename T, int G, int NV>
+__global__ void __launch_bounds__(256) diff_dw_kernel(AttnArgs a) {
+  constexpr int U = 4;
+  const Item it = find_item(a.w);
+  const int gs = a.w.gs, lane = threadIdx.x & (gs - 1);
+  const int c = lane % G, slot = lane / G, slots = gs / G, vch = a.dvp / 8;
+  const bool has = it.row >= 0;
+  const int64_t row = has ? it.row : 0;
+  Raw<T> g[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    g[i] = zero8<T>();
+    if (has && c + i * G < vch)
+      g[i] = load8((const T*)a.go + row * a.ldgo + (int64_t)it.head * a.dvp + (c + i * G) * 8);
+  }
+  const float4 st = a.stat[(int64_t)it.head * a.w.rows + row];
+  const T* vb = (const T*)a.v + (int64_t)it.head * a.dvp + c * 8;
+  const int64_t at = (int64_t)it.head * a.E + it.beg;
+  const int n = has ? it.end - it.beg : 0;
+  const int turns = wave_max((n + slots * U - 1) / (slots * U));
+  float d1 = 0.f, d2 = 0.f;
+  for (int t = 0; t < turns; ++t) {
+    Raw<T> v[U][NV];
+    float2 x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int o = (t * U + u) * slots + slot;
+      const int e = o < n ? o : 0;
+      const int64_t j = n > 0 ? a.col[it.beg + e] : 0;
+      x[u] = n > 0 ? a.S[at + e] : make_float2(-kInf, -kInf);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        v[u][i] = zero8<T>();
+        if (c + i * G < vch) v[u][i] = load8(vb + j * a.ldv + i * G * 8);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int o = (t * U + u) * slots + slot;
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) s = dot8(g[i], v[u][i], s);
+      s = edge_sum<G>(s);
+      if (x[u].x == -kInf && x[u].y == -kInf) s = 0.f;   // shut: its value does not count
+      const float2 p = weights(x[u], st);
+      if (o < n) {
+        d1 = fmaf(p.x, s, d1);
+        d2 = fmaf(p.y, s, d2);
+        if (c == 0) a.dw[at + o] = s;
+      }
+    }
+  }
+  d1 = slots_sum<G>(d1, gs);
+  d2 = slots_sum<G>(d2, gs);
+  if (!has || lane != 0) return;
+  if (it.slot >= 0)
+    *(float2*)(a.part + (it.slot * a.w.heads + it.head) * 2) = make_float2(d1, d2);
+  else
+    a.D[(int64_t)it.head * a.w.rows + row] = make_float2(d1, d2);
+}
+__global__ void __launch_bounds__(256) diff_dw_join_kernel(AttnArgs a) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t pc = i / a.w.heads;
+  const int head = (int)(i - pc * a.w.heads);
+  if (pc >= a.w.hub_bound || pc >= *a.w.hub_count) return;
+  const int32_t* hp = a.w.hubs + 4 * pc;
+  if (hp[1] != 0) return;
+  float2 d = make_float2(0.f, 0.f);
+  for (int k = 0; k < hp[2]; ++k) {
+    const float2 p = *(const float2*)(a.part + ((pc + k) * a.w.heads + head) * 2);
+    d.x += p.x;
+    d.y += p.y;
+  }
+  a.D[(int64_t)head * a.w.rows + hp[0]] = d;
+}
+
+// B: gq of every row, and each edge's record for C and the bias.
+template <typename T, int G>
+__global__ void __launch_bounds__(256) diff_gq_kernel(AttnArgs a) {
+  constexpr int U = 4;
+  const Item it = find_item(a.w);
+  const int gs = a.w.gs, lane = threadIdx.x & (gs - 1);
+  const int c = lane % G, slot = lane / G, slots = gs / G, dch = a.dp / 8;
+  const bool has = it.row >= 0;
+  const int64_t row = has ? it.row : 0, sr = (int64_t)it.head * a.w.rows + row;
+  const float4 st = a.stat[sr];
+  const float2 D = a.D[sr];
+  const float lam = a.lam[it.head];
+  const T* kb = (const T*)a.k + (int64_t)it.head * 2 * a.dp + c * 8;
+  const int64_t at = (int64_t)it.head * a.E + it.beg;
+  const int n = has ? it.end - it.beg : 0;
+  const int turns = wave_max((n + slots * U - 1) / (slots * U));
+  float g1[8] = {}, g2[8] = {};
+  for (int t = 0; t < turns; ++t) {
+    Raw<T> k1[U], k2[U];
+    float2 x[U];
+    float dw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int o = (t * U + u) * slots + slot;
+      const int e = o < n ? o : 0;
+      const int64_t j = n > 0 ? a.col[it.beg + e] : 0;
+      x[u] = o < n ? a.S[at + e] : make_float2(-kInf, -kInf);
+      dw[u] = n > 0 ? a.dw[at + e] : 0.f;
+      k1[u] = k2[u] = zero8<T>();
+      if (c < dch) {
+        k1[u] = load8(kb + j * a.ldk);
+        k2[u] = load8(kb + j * a.ldk + a.dp);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int o = (t * U + u) * slots + slot;
+      const bool shut = x[u].x == -kInf && x[u].y == -kInf;   // or past the end
+      const float2 p = weights(x[u], st);
+      const float x1 = shut ? 0.f : p.x * (dw[u] - D.x);
+      const float x2 = shut ? 0.f : -lam * p.y * (dw[u] - D.y);
+      if (c == 0 && o < n)
+        a.rec[at + o] = make_float4(x1 * a.scale, x2 * a.scale, shut ? 0.f : p.x - lam * p.y,
+                                    x1 + x2);
+      axpy8(x1, keep8(!shut, k1[u]), g1);
+      axpy8(x2, keep8(!shut, k2[u]), g2);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    g1[i] = slots_sum<G>(g1[i], gs) * a.scale;
+    g2[i] = slots_sum<G>(g2[i], gs) * a.scale;
+  }
+  if (!has || slot != 0 || !a.gq) return;
+  if (it.slot >= 0) {
+    float* p = a.part + (it.slot * a.w.heads + it.head) * a.part_width;
+    store8(p, c * 8, a.dp, true, g1);
+    store8(p + a.dp, c * 8, a.dp, true, g2);
+  } else {
+    T* gq = (T*)a.gq + (row * a.w.heads + it.head) * 2 * a.d;
+    store8(gq, c * 8, a.d, a.d == a.dp, g1);
+    store8(gq + a.d, c * 8, a.d, a.d == a.dp, g2);
+  }
+}
+
+// C: gk and gv of every source from its out-edges (CSR w.rowptr = srowptr, col = scol).
+template <typename T, int G, int NV>
+__global__ void __launch_bounds__(256) diff_gkv_kernel(AttnArgs a) {
+  constexpr int U = 2;
+  const Item it = find_item(a.w);
+  const int gs = a.w.gs, lane = threadIdx.x & (gs - 1);
+  const int c = lane % G, slot = lane / G, slots = gs / G;
+  const int dch = a.dp / 8, vch = a.dvp / 8;
+  const bool has = it.row >= 0;
+  const int64_t row = has ? it.row : 0;
+  const T* qb = (const T*)a.q + (int64_t)it.head * 2 * a.dp + c * 8;
+  const T* gb = (const T*)a.go + (int64_t)it.head * a.dvp + c * 8;
+  const float4* rec = a.rec + (int64_t)it.head * a.E;
+  const int n = has ? it.end - it.beg : 0;
+  const int turns = wave_max((n + slots * U - 1) / (slots * U));
+  float g1[8] = {}, g2[8] = {}, gv[NV][8] = {};
+  for (int t = 0; t < turns; ++t) {
+    Raw<T> q1[U], q2[U], go[U][NV];
+    float4 r[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int o = (t * U + u) * slots + slot;
+      const int e = it.beg + (o < n ? o : 0);
+      const int64_t i = n > 0 ? a.col[e] : 0;
+      r[u] = o < n ? rec[a.seid[e]] : make_float4(0.f, 0.f, 0.f, 0.f);
+      q1[u] = q2[u] = zero8<T>();
+      if (c < dch) {
+        q1[u] = load8(qb + i * a.ldq);
+        q2[u] = load8(qb + i * a.ldq + a.dp);
+      }
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        go[u][k] = zero8<T>();
+        if (c + k * G < vch) go[u][k] = load8(gb + i * a.ldgo + k * G * 8);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      // a shut edge (or one past the end) is all zeros: what it points at does not count
+      const bool keep = r[u].x != 0.f || r[u].y != 0.f || r[u].z != 0.f;
+      axpy8(r[u].x, keep8(keep, q1[u]), g1);
+      axpy8(r[u].y, keep8(keep, q2[u]), g2);
+#pragma unroll
+      for (int k = 0; k < NV; ++k) axpy8(r[u].z, keep8(keep, go[u][k]), gv[k]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    g1[i] = slots_sum<G>(g1[i], gs);
+    g2[i] = slots_sum<G>(g2[i], gs);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) gv[k][i] = slots_sum<G>(gv[k][i], gs);
+  }
+  if (!has || slot != 0) return;
+  if (it.slot >= 0) {
+    float* p = a.part + (it.slot * a.w.heads + it.head) * a.part_width;
+    store8(p, c * 8, a.dp, true, g1);
+    store8(p + a.dp, c * 8, a.dp, true, g2);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) store8(p + 2 * a.dp, (c + k * G) * 8, a.dvp, true, gv[k]);
+    return;
+  }
+  const int64_t rh = row * a.w.heads + it.head;
+  if (a.gk) {
+    T* gk = (T*)a.gk + rh * 2 * a.d;
+    store8(gk, c * 8, a.d, a.d == a.dp, g1);
+    store8(gk + a.d, c * 8, a.d, a.d == a.dp, g2);
+  }
+  if (a.gv) {
+    T* out = (T*)a.gv + rh * a.dv;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) store8(out, (c + k * G) * 8, a.dv, a.dv == a.dvp, gv[k]);
+  }
+}
+// A hub's gradient pieces summed in order: [two maps of dp | dvp] columns, one thread a column.
+template <typename T>
+__global__ void __launch_bounds__(256) diff_grad_join_kernel(AttnArgs a, T* maps, T* values) {
+  const int64_t pc = blockIdx.x / a.w.heads;
+  const int head = (int)(blockIdx.x - pc * a.w.heads);
+  if (pc >= *a.w.hub_count) return;
+  const int32_t* hp = a.w.hubs + 4 * pc;
+  if (hp[1] != 0) return;
+  const int64_t rh = (int64_t)hp[0] * a.w.heads + head;
+  const int64_t step = (int64_t)a.w.heads * a.part_width;
+  for (int x = threadIdx.x; x < a.part_width; x += 256) {
+    const float* p = a.part + (pc * a.w.heads + head) * a.part_width + x;
+    float s = 0.f;
+#pragma unroll 8
+    for (int k = 0; k < hp[2]; ++k) s += p[k * step];
+    if (x < 2 * a.dp) {
+      const int m = x >= a.dp, y = x - m * a.dp;
+      if (maps && y < a.d) maps[(rh * 2 + m) * a.d + y] = (T)s;
+    } else if (values && x - 2 * a.dp < a.dv) {
+      values[rh * a.dv + x - 2 * a.dp] = (T)s;
+    }
+  }
+}
+
+// glam[h] = -sum of D_2 over the rows: a workgroup per (run of rows, head), then the runs in order.
+constexpr int kLamRuns = 64;
+__global__ void __launch_bounds__(1024) diff_lam_kernel(const float2* D, int64_t rows, int64_t per,
+                                                        float* part, float* glam) {
+  __shared__ float red[16];
+  const int h = blockIdx.y;
+  const int64_t r0 = blockIdx.x * per, r1 = min(rows, r0 + per);
+  float s = 0.f;
+#pragma unroll 4
+  for (int64_t r = r0 + threadIdx.x; r < r1; r += 1024) s += D[h * rows + r].y;
+  s = group_sum<64>(s);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x) return;
+  s = 0.f;
+  for (int i = 0; i < 16; ++i) s += red[i];
+  if (gridDim.x == 1) glam[h] = -s;
+  else part[h * gridDim.x + blockIdx.x] = s;
+}
+__global__ void __launch_bounds__(64) diff_lam_join_kernel(const float* part, int runs,
+                                                           float* glam) {
+  const float s = group_sum<64>(threadIdx.x < runs ? part[blockIdx.x * runs + threadIdx.x] : 0.f);
+  if (threadIdx.x == 0) glam[blockIdx.x] = -s;
+}
+
+// gbias: each lane adds its edges' dx_1 + dx_2 into a column of its own of an LDS table [bucket]
+// [lane] (no two lanes share a word, so no atomics and one order), a wave per run of slots of one
+// head; the lanes' columns, then the runs, are summed in order.
+__global__ void __launch_bounds__(64) diff_bias_kernel(const float4* rec, const uint8_t* bucket,
+                                                       const int32_t* rowptr, int64_t num_nodes,
+                                                       int64_t E, int64_t per, int nb,
+                                                       float* part) {
+  extern __shared__ float hist[];   // [nb][64]
+  const int lane = threadIdx.x, h = blockIdx.y;
+  for (int b = 0; b < nb; ++b) hist[b * 64 + lane] = 0.f;
+  const int64_t end = min((int64_t)rowptr[num_nodes], (int64_t)(blockIdx.x + 1) * per);
+  const float* r = (const float*)(rec + h * E) + 3;
+  int64_t e = blockIdx.x * per + lane;
+  for (; e + 192 < end; e += 256) {
+    float x[4];
+    int b[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      x[u] = r[4 * (e + 64 * u)];
+      b[u] = bucket[e + 64 * u];
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) hist[b[u] * 64 + lane] += x[u];
+  }
+  for (; e < end; e += 64) hist[(int)bucket[e] * 64 + lane] += r[4 * e];
+  float* p = part + ((int64_t)h * gridDim.x + blockIdx.x) * nb;
+  for (int b = 0; b < nb; ++b) {
+    const float s = group_sum<64>(hist[b * 64 + lane]);
+    if (lane == 0) p[b] = s;
+  }
+}
+__global__ void __launch_bounds__(64) diff_bias_join_kernel(const float* part, int runs, int nb,
+                                                            int heads, float* gbias) {
+  const int b = blockIdx.x, h = blockIdx.y;
+  float s = 0.f;
+  for (int i = threadIdx.x; i < runs; i += 64) s += part[((int64_t)h * runs + i) * nb + b];
+  s = group_sum<64>(s);
+  if (threadIdx.x == 0) gbias[b * heads + h] = s;
+}
+
+// ------------------------------------------------------------------ buckets and packing
+struct BucketArgs {
+  const int32_t *rowptr, *col, *rowidx;
+  const int64_t* nodes;
+  int64_t num_nodes, n_nodes;
+  const void* pos;
+  int pos64, exact, n_bounds, bidirectional;
+  int64_t bounds[kMaxBuckets / 2];
+  uint8_t* bucket;
+};
+__device__ inline uint8_t bucket_of(const BucketArgs& a, const int64_t* bounds, int64_t src,
+                                    int64_t dst) {
+  auto at = [&](int64_t n) {
+    return a.pos64 ? ((const int64_t*)a.pos)[n] : (int64_t)((const int32_t*)a.pos)[n];
+  };
+  const int64_t s = at(src), d = at(dst);
+  // as unsigned: the difference of any two int64 fits
+  uint64_t away = s > d ? (uint64_t)s - (uint64_t)d : (uint64_t)d - (uint64_t)s;
+  int b = 0;
+  if (a.bidirectional) b = s > d ? a.exact + a.n_bounds + 1 : 0;
+  else if (s > d) away = 0;
+  if (away < (uint64_t)a.exact) return (uint8_t)(b + (int)away);
+  int lo = 0, hi = a.n_bounds;   // the number of bounds <= away
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if ((uint64_t)bounds[mid] <= away) lo = mid + 1;
+    else hi = mid;
+  }
+  return (uint8_t)(b + a.exact + lo);
+}
+// One thread a slot; with nodes, a workgroup row of the grid walks one node's slots.
+__global__ void __launch_bounds__(256) relative_bucket_kernel(BucketArgs a) {
+  __shared__ int64_t bounds[kMaxBuckets / 2];
+  if ((int)threadIdx.x < a.n_bounds) bounds[threadIdx.x] = a.bounds[threadIdx.x];
+  __syncthreads();
+  if (!a.nodes) {
+    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (e < a.rowptr[a.num_nodes]) a.bucket[e] = bucket_of(a, bounds, a.col[e], a.rowidx[e]);
+    return;
+  }
+  for (int64_t i = blockIdx.y; i < a.n_nodes; i += gridDim.y) {
+    const int64_t n = a.nodes[i];
+    if (n < 0 || n >= a.num_nodes) continue;
+    const int end = a.rowptr[n + 1];
+    for (int64_t e = (int64_t)a.rowptr[n] + blockIdx.x * 256 + threadIdx.x; e < end;
+         e += (int64_t)gridDim.x * 256)
+      a.bucket[e] = bucket_of(a, bounds, a.col[e], n);
+  }
+}
+
+struct PackArgs {
+  const void* src[3];
+  void* dst[3];
+  int64_t ld[3], n[3];   // n: 8-element chunks of the packed tensor
+  int groups[3], width[3];
+};
+template <typename T>
+__global__ void __launch_bounds__(256) pack_heads_kernel(PackArgs a) {
+  const int t = blockIdx.y;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= a.n[t]) return;
+  const int w = a.width[t], chunks = (w + 7) / 8;
+  const int64_t g = i / chunks, row = g / a.groups[t];
+  const int c = (int)(i - g * chunks) * 8;
+  const T* s = (const T*)a.src[t] + row * a.ld[t] + (g - row * a.groups[t]) * w;
+  Pack<T, 8> x;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) x.v[j] = c + j < w ? s[c + j] : (T)0.f;
+  *reinterpret_cast<Pack<T, 8>*>((T*)a.dst[t] + i * 8) = x;
+}
+
+// ------------------------------------------------------------------ launches
+struct Geom {
+  int G, NV;
+};
+// The smallest G lanes that hold both maps' d in one chunk a lane and dv in at most two.
+Geom attn_geom(int d, int dv) {
+  const int dch = (int)ceil_div(d, 8), vch = (int)ceil_div(dv, 8);
+  int G = 1;
+  while (G < dch || 2 * G < vch) G <<= 1;
+  return {G, vch > G ? 2 : 1};
+}
+template <typename F>
+void with_geom(const Geom& g, F&& f) {
+  auto nv = [&](auto G) {
+    if (g.NV == 1) f(G, std::integral_constant<int, 1>());
+    else f(G, std::integral_constant<int, 2>());
+  };
+  switch (g.G) {
+    case 1: nv(std::integral_constant<int, 1>()); break;
+    case 2: nv(std::integral_constant<int, 2>()); break;
+    case 4: nv(std::integral_constant<int, 4>()); break;
+    case 8: nv(std::integral_constant<int, 8>()); break;
+    case 16: nv(std::integral_constant<int, 16>()); break;
+    default: nv(std::integral_constant<int, 32>()); break;
+  }
+}
+// Lanes of a row: 16, 32 or 64, at least G; `per_row` = its average number of edges.
+int row_lanes(int G, double per_row, int edges_per_slot) {
+  int gs = 16;
+  while (gs < 64 && (gs < G || (double)(gs / G) * edges_per_slot < per_row)) gs <<= 1;
+  return gs;
+}
+
+// The plain rows' grid (and the pieces' blocks ahead of it).
+unsigned plan_rows(Work& w, int64_t rows, int heads, int gs, const int32_t* rowptr, int hub_edges,
+                   const int32_t* hubs, const int32_t* hub_count, int64_t hub_bound) {
+  w = Work{};
+  w.rows = w.num_nodes = rows;
+  w.heads = heads;
+  w.gs = gs;
+  w.rowptr = rowptr;
+  const int per_block = 256 / gs;
+  // units of kChunk rows; fewer where that would leave XCDs without one
+  int64_t chunk = std::min<int64_t>(kChunk, ceil_div(rows * heads, 64));
+  chunk = std::max<int64_t>(round_up(chunk, per_block), per_block);
+  w.chunk = (int)chunk;
+  w.units = ceil_div(rows, chunk) * heads;
+  w.blocks_per_unit = (int)(chunk / per_block);
+  if (hub_edges > 0 && hub_bound > 0) {
+    w.hub_edges = hub_edges;
+    w.hubs = hubs;
+    w.hub_count = hub_count;
+    w.hub_bound = hub_bound;
+    w.hub_blocks = ceil_div(hub_bound * heads, per_block);
+  }
+  return (unsigned)(w.hub_blocks + round_up(w.units, 8) * w.blocks_per_unit);
+}
+
+struct Dims {
+  int dtype, heads, d, dv, dp, dvp;
+};
+int check_dims(const char* what, int dtype, int heads, int d, int dv, int64_t E, int64_t rows) {
+  GATX_REQUIRE(dtype_ok(dtype), "%s: unknown dtype %d", what, dtype);
+  GATX_REQUIRE(heads >= 1 && heads <= 65535, "%s: %d heads", what, heads);
+  GATX_REQUIRE(d >= 1 && d <= kMaxD && dv >= 1 && dv <= kMaxDv,
+               "%s: head widths d = %d (1..%d), dv = %d (1..%d)", what, d, kMaxD, dv, kMaxDv);
+  GATX_REQUIRE(E >= 0 && E < (1ll << 31) && rows >= 0 && rows < (1ll << 31), "%s: bad graph size",
+               what);
+  return 0;
+}
+bool chunked(int dtype, const void* p, int64_t ld) {
+  return aligned16(p) && ld * dtype_size(dtype) % 16 == 0;
+}
+#define GATX_GRID(blocks, what)                                                             \
+  GATX_REQUIRE((blocks) < (1ll << 31), "%s: too many work items for one launch", what)
+
+}  // namespace
+}  // namespace gatx
+
+using namespace gatx;
+
+extern "C" int gatx_relative_buckets(const int32_t* rowptr, const int32_t* col,
+                                     const int32_t* rowidx, int64_t E, int64_t num_nodes,
+                                     const int64_t* nodes, int64_t n_nodes, const void* pos,
+                                     int pos_is64, int exact, const int64_t* bounds, int n_bounds,
+                                     int bidirectional, uint8_t* bucket, gatx_stream_t s) {
+  GATX_REQUIRE(exact >= 1 && n_bounds >= 0 && n_bounds < kMaxBuckets / 2 &&
+               (exact + n_bounds + 1) * (bidirectional ? 2 : 1) <= kMaxBuckets,
+               "relative_buckets: %d exact buckets and %d bounds (at most %d in all)", exact,
+               n_bounds, kMaxBuckets);
+  GATX_REQUIRE(n_bounds == 0 || bounds, "relative_buckets: null bounds");
+  if (E == 0 || num_nodes == 0 || (nodes && n_nodes == 0)) return 0;
+  GATX_REQUIRE(rowptr && col && pos && bucket && (nodes || rowidx),
+               "relative_buckets: null buffer");
+  BucketArgs a = {};
+  a.rowptr = rowptr; a.col = col; a.rowidx = rowidx; a.nodes = nodes; a.num_nodes = num_nodes;
+  a.n_nodes = n_nodes; a.pos = pos; a.pos64 = pos_is64; a.exact = exact; a.n_bounds = n_bounds;
+  a.bidirectional = bidirectional; a.bucket = bucket;
+  for (int i = 0; i < n_bounds; ++i) a.bounds[i] = bounds[i];
+  dim3 grid((unsigned)ceil_div(E, 256));
+  if (nodes)
+    grid = dim3((unsigned)std::min<int64_t>(ceil_div(E, 256), std::max<int64_t>(1, 512 / n_nodes)),
+                (unsigned)std::min<int64_t>(n_nodes, 32768));
+  relative_bucket_kernel<<<grid, 256, 0, (hipStream_t)s>>>(a);
+  GATX_LAUNCH_CHECK("relative_buckets");
+  return 0;
+}
+
+extern "C" int gatx_diff_attention_pack(int dtype, int64_t rows, int64_t keys, int heads, int d,
+                                        int dv, const void* q, int64_t ldq, void* qp,
+                                        const void* k, int64_t ldk, void* kp, const void* v,
+                                        int64_t ldv, void* vp, gatx_stream_t s) {
+  GATX_CALL(check_dims("diff_attention_pack", dtype, heads, d, dv, 0, std::max(rows, keys)));
+  PackArgs a = {};
+  int t = 0;
+  int64_t most = 0;
+  auto add = [&](const void* src, int64_t ld, void* dst, int64_t n, int groups, int width) {
+    if (!src || n == 0) return;
+    a.src[t] = src; a.dst[t] = dst; a.ld[t] = ld; a.groups[t] = groups; a.width[t] = width;
+    a.n[t] = n * groups * ceil_div(width, 8);
+    most = std::max(most, a.n[t]);
+    ++t;
+  };
+  add(q, ldq, qp, rows, 2 * heads, d);
+  add(k, ldk, kp, keys, 2 * heads, d);
+  add(v, ldv, vp, keys, heads, dv);
+  if (t == 0) return 0;
+  for (int i = 0; i < t; ++i)
+    GATX_REQUIRE(a.dst[i] && aligned16(a.dst[i]), "diff_attention_pack: bad destination");
+  GATX_GRID(ceil_div(most, 256), "diff_attention_pack");
+  const dim3 grid((unsigned)ceil_div(most, 256), t);
+  with_dtype(dtype, [&](auto x) {
+    pack_heads_kernel<decltype(x)><<<grid, 256, 0, (hipStream_t)s>>>(a);
+    return 0;
+  });
+  GATX_LAUNCH_CHECK("diff_attention_pack");
+  return 0;
+}
+
+extern "C" size_t gatx_diff_attention_part_bytes(int64_t slots, int heads, int dvp) {
+  return sizeof(float) * (size_t)std::max<int64_t>(slots, 0) * heads * (2 * dvp + 4);
+}
+
+extern "C" int gatx_diff_attention(int dtype, const void* q, int64_t ldq, const void* k,
+                                   int64_t ldk, const void* v, int64_t ldv, int heads, int d,
+                                   int dv, const int32_t* rowptr, const int32_t* col, int64_t E,
+                                   int64_t rows, int64_t num_nodes, const int64_t* nodes,
+                                   int pieces, float scale, const float* lam, const float* bias,
+                                   const uint8_t* bucket, void* out, float* S, float* stat,
+                                   int hub_edges, const int32_t* hubs, const int32_t* hub_count,
+                                   int64_t hub_bound, void* part, size_t part_bytes,
+                                   gatx_stream_t s) {
+  GATX_CALL(check_dims("diff_attention", dtype, heads, d, dv, E, std::max(rows, num_nodes)));
+  if (rows == 0) return 0;
+  GATX_REQUIRE(q && k && v && rowptr && col && lam && out, "diff_attention: null buffer");
+  GATX_REQUIRE(nodes || rows == num_nodes, "diff_attention: a row for every node without nodes");
+  GATX_REQUIRE(num_nodes > 0, "diff_attention: no nodes");
+  GATX_REQUIRE(chunked(dtype, q, ldq) && chunked(dtype, k, ldk) && chunked(dtype, v, ldv),
+               "diff_attention: rows of q, k, v must be 16-byte aligned (pack them)");
+  GATX_REQUIRE(aligned16(out), "diff_attention: out must be 16-byte aligned");
+  GATX_REQUIRE(!bias == !bucket, "diff_attention: bias and bucket go together");
+  GATX_REQUIRE(!S == !stat && !(S && nodes), "diff_attention: S and stat go together, not with nodes");
+  AttnArgs a = {};
+  a.q = q; a.k = k; a.v = v; a.ldq = ldq; a.ldk = ldk; a.ldv = ldv;
+  a.d = d; a.dv = dv; a.dp = (int)round_up(d, 8); a.dvp = (int)round_up(dv, 8);
+  a.col = col; a.E = E; a.scale = scale; a.lam = lam; a.bias = bias; a.bucket = bucket;
+  a.S = (float2*)S; a.stat = (float4*)stat; a.out = out;
+  a.part = (float*)part; a.part_width = 2 * a.dvp + 4;
+  const Geom g = attn_geom(d, dv);
+  const double per_row = (double)E / (double)num_nodes;
+  int64_t blocks, slots = 0;
+  if (nodes) {
+    GATX_REQUIRE(pieces >= 1 && pieces <= 4096, "diff_attention: 1..4096 pieces");
+    a.w.rows = rows; a.w.num_nodes = num_nodes; a.w.heads = heads; a.w.rowptr = rowptr;
+    a.w.nodes = nodes; a.w.pieces = pieces;
+    a.w.gs = pieces > 1 ? 64 : row_lanes(g.G, per_row, 4);
+    slots = pieces > 1 ? rows * pieces : 0;
+    blocks = ceil_div(rows * heads * pieces, 256 / a.w.gs);
+  } else {
+    GATX_REQUIRE(hub_edges == 0 || (hubs && hub_count), "diff_attention: null hub plan");
+    blocks = plan_rows(a.w, rows, heads, row_lanes(g.G, per_row, 4), rowptr, hub_edges, hubs,
+                       hub_count, hub_bound);
+    slots = a.w.hub_blocks ? hub_bound : 0;
+  }
+  GATX_GRID(blocks, "diff_attention");
+  GATX_REQUIRE(slots == 0 || (part && part_bytes >= gatx_diff_attention_part_bytes(slots, heads, a.dvp)),
+               "diff_attention: workspace too small");
+  hipStream_t st = (hipStream_t)s;
+  with_dtype(dtype, [&](auto t) {
+    using T = decltype(t);
+    with_geom(g, [&](auto G, auto NV) {
+      constexpr int kG = decltype(G)::value, kNV = decltype(NV)::value;
+      if (bias && S) diff_forward_kernel<T, kG, kNV, true, true><<<(unsigned)blocks, 256, 0, st>>>(a);
+      else if (bias) diff_forward_kernel<T, kG, kNV, true, false><<<(unsigned)blocks, 256, 0, st>>>(a);
+      else if (S) diff_forward_kernel<T, kG, kNV, false, true><<<(unsigned)blocks, 256, 0, st>>>(a);
+      else diff_forward_kernel<T, kG, kNV, false, false><<<(unsigned)blocks, 256, 0, st>>>(a);
+    });
+    return 0;
+  });
+  GATX_LAUNCH_CHECK("diff_attention");
+  if (slots > 0) {
+    const int64_t joins = (nodes ? rows : hub_bound) * heads;
+    GATX_GRID(joins, "diff_attention");
+    with_dtype(dtype, [&](auto t) {
+      diff_join_kernel<decltype(t)><<<(unsigned)joins, 1024, sizeof(float) * 8 * a.dvp, st>>>(a);
+      return 0;
+    });
+    GATX_LAUNCH_CHECK("diff_attention_join");
+  }
+  return 0;
+}
+
+namespace {
+// Runs of slots of the bias gradient: enough waves to fill the chip, at least 1024 slots each.
+int64_t bias_runs(int64_t E) { return std::max<int64_t>(1, std::min<int64_t>(512, E / 1024)); }
+struct BackwardLayout {
+  size_t dw, D, rec, lam, bias, part, total;
+};
+BackwardLayout backward_layout(int64_t N, int64_t E, int H, int dp, int dvp, int nb,
+                               int64_t hub_bound, int64_t src_hub_bound) {
+  BackwardLayout l = {};
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t here = at;
+    at += (bytes + 255) / 256 * 256;
+    return here;
+  };
+  const size_t he = (size_t)H * E, hn = (size_t)H * N;
+  l.rec = take(he * sizeof(float4));
+  l.dw = take(he * sizeof(float));
+  l.D = take(hn * sizeof(float2));
+  l.lam = take(sizeof(float) * kLamRuns * H);
+  l.bias = take(nb ? sizeof(float) * bias_runs(E) * H * nb : 0);
+  l.part = take(sizeof(float) * std::max((size_t)hub_bound * H * (2 * dp),
+                                         (size_t)src_hub_bound * H * (2 * dp + dvp)));
+  l.total = at;
+  return l;
+}
+}  // namespace
+
+extern "C" size_t gatx_diff_attention_backward_workspace_bytes(int64_t N, int64_t E, int heads,
+                                                               int d, int dv, int n_buckets,
+                                                               int64_t hub_bound,
+                                                               int64_t src_hub_bound) {
+  return backward_layout(N, E, heads, (int)round_up(d, 8), (int)round_up(dv, 8), n_buckets,
+                         hub_bound, src_hub_bound).total;
+}
+
+extern "C" int gatx_diff_attention_backward(
+    int dtype, const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv,
+    const void* go, int64_t ldgo, int heads, int d, int dv, const int32_t* rowptr,
+    const int32_t* col, const int32_t* srowptr, const int32_t* scol, const int32_t* seid, int64_t E,
+    int64_t N, float scale, const float* lam, const uint8_t* bucket, int n_buckets, const float* S,
+    const float* stat, void* gq, void* gk, void* gv, float* glam, float* gbias, int hub_edges,
+    const int32_t* hubs, const int32_t* hub_count, int64_t hub_bound, const int32_t* src_hubs,
+    const int32_t* src_hub_count, int64_t src_hub_bound, void* workspace, size_t workspace_bytes,
+    gatx_stream_t s) {
+  GATX_CALL(check_dims("diff_attention_backward", dtype, heads, d, dv, E, N));
+  GATX_REQUIRE(n_buckets >= 0 && n_buckets <= kMaxBuckets, "diff_attention_backward: %d buckets",
+               n_buckets);
+  GATX_REQUIRE(!gbias || (bucket && n_buckets > 0), "diff_attention_backward: null bucket");
+  hipStream_t st = (hipStream_t)s;
+  if (N == 0) {
+    if (glam) zero_words_kernel<<<(unsigned)ceil_div(heads, 64), 64, 0, st>>>((uint32_t*)glam, heads);
+    if (gbias)
+      zero_words_kernel<<<(unsigned)ceil_div(n_buckets * heads, 64), 64, 0, st>>>(
+          (uint32_t*)gbias, n_buckets * heads);
+    GATX_LAUNCH_CHECK("diff_attention_backward zero");
+    return 0;
+  }
+  const bool by_source = gk || gv;
+  GATX_REQUIRE(aligned16(gq) && aligned16(gk) && aligned16(gv),
+               "diff_attention_backward: gradients must be 16-byte aligned");
+  GATX_REQUIRE(q && k && v && go && rowptr && col && lam && S && stat,
+               "diff_attention_backward: null buffer");
+  GATX_REQUIRE(!by_source || (srowptr && scol && seid), "diff_attention_backward: null transpose");
+  GATX_REQUIRE(chunked(dtype, q, ldq) && chunked(dtype, k, ldk) && chunked(dtype, v, ldv) &&
+               chunked(dtype, go, ldgo),
+               "diff_attention_backward: rows of q, k, v, go must be 16-byte aligned (pack them)");
+  GATX_REQUIRE(hub_edges == 0 || (hubs && hub_count && (!by_source || (src_hubs && src_hub_count))),
+               "diff_attention_backward: null hub plan");
+  const int dp = (int)round_up(d, 8), dvp = (int)round_up(dv, 8);
+  const BackwardLayout l =
+      backward_layout(N, E, heads, dp, dvp, gbias ? n_buckets : 0, hub_bound, src_hub_bound);
+  GATX_REQUIRE(workspace && workspace_bytes >= l.total,
+               "diff_attention_backward: workspace too small");
+  char* ws = (char*)workspace;
+  AttnArgs a = {};
+  a.q = q; a.k = k; a.v = v; a.go = go; a.ldq = ldq; a.ldk = ldk; a.ldv = ldv; a.ldgo = ldgo;
+  a.d = d; a.dv = dv; a.dp = dp; a.dvp = dvp; a.col = col; a.E = E; a.scale = scale; a.lam = lam;
+  a.S = (float2*)const_cast<float*>(S); a.stat = (float4*)const_cast<float*>(stat);
+  a.dw = (float*)(ws + l.dw); a.D = (float2*)(ws + l.D); a.rec = (float4*)(ws + l.rec);
+  a.part = (float*)(ws + l.part);
+  a.gq = gq; a.gk = gk; a.gv = gv;
+  const Geom g = attn_geom(d, dv);
+  const double per_row = (double)E / (double)N;
+  const int gs = row_lanes(g.G, per_row, 4);
+  // A
+  int64_t blocks = plan_rows(a.w, N, heads, gs, rowptr, hub_edges, hubs, hub_count, hub_bound);
+  GATX_GRID(blocks, "diff_attention_backward");
+  with_dtype(dtype, [&](auto t) {
+    using T = decltype(t);
+    with_geom(g, [&](auto G, auto NV) {
+      diff_dw_kernel<T, decltype(G)::value, decltype(NV)::value>
+          <<<(unsigned)blocks, 256, 0, st>>>(a);
+    });
+    return 0;
+  });
+  GATX_LAUNCH_CHECK("diff_attention_dw");
+  if (a.w.hub_blocks) {
+    diff_dw_join_kernel<<<(unsigned)ceil_div(hub_bound * heads, 256), 256, 0, st>>>(a);
+    GATX_LAUNCH_CHECK("diff_attention_dw_join");
+  }
+  if (glam) {
+    const int runs = (int)std::min<int64_t>(kLamRuns, ceil_div(N, 8192));
+    float* lp = (float*)(ws + l.lam);
+    diff_lam_kernel<<<dim3(runs, heads), 1024, 0, st>>>(a.D, N, ceil_div(N, runs), lp, glam);
+    GATX_LAUNCH_CHECK("diff_attention_lam");
+    if (runs > 1) diff_lam_join_kernel<<<heads, 64, 0, st>>>(lp, runs, glam);
+    GATX_LAUNCH_CHECK("diff_attention_lam_join");
+  }
+  // B
+  if (gq || by_source || gbias) {
+    a.part_width = 2 * dp;
+    with_dtype(dtype, [&](auto t) {
+      using T = decltype(t);
+      with_geom(Geom{g.G, 1}, [&](auto G, auto) {
+        diff_gq_kernel<T, decltype(G)::value><<<(unsigned)blocks, 256, 0, st>>>(a);
+      });
+      return 0;
+    });
+    GATX_LAUNCH_CHECK("diff_attention_gq");
+    if (a.w.hub_blocks && gq) {
+      GATX_GRID(hub_bound * heads, "diff_attention_backward");
+      with_dtype(dtype, [&](auto t) {
+        using T = decltype(t);
+        diff_grad_join_kernel<T><<<(unsigned)(hub_bound * heads), 256, 0, st>>>(a, (T*)gq, nullptr);
+        return 0;
+      });
+      GATX_LAUNCH_CHECK("diff_attention_gq_join");
+    }
+  }
+  if (gbias) {
+    const int64_t runs = bias_runs(E);
+    float* bp = (float*)(ws + l.bias);
+    diff_bias_kernel<<<dim3((unsigned)runs, heads), 64, sizeof(float) * 64 * n_buckets, st>>>(
+        a.rec, bucket, rowptr, N, E, ceil_div(E, runs), n_buckets, bp);
+    GATX_LAUNCH_CHECK("diff_attention_bias");
+    diff_bias_join_kernel<<<dim3(n_buckets, heads), 64, 0, st>>>(bp, (int)runs, n_buckets, heads,
+                                                                 gbias);
+    GATX_LAUNCH_CHECK("diff_attention_bias_join");
+  }
+  // C
+  if (by_source) {
+    a.col = scol;
+    a.seid = seid;
+    a.part_width = 2 * dp + dvp;
+    blocks = plan_rows(a.w, N, heads, gs, srowptr, hub_edges, src_hubs, src_hub_count,
+                       src_hub_bound);
+    GATX_GRID(blocks, "diff_attention_backward");
+    with_dtype(dtype, [&](auto t) {
+      using T = decltype(t);
+      with_geom(g, [&](auto G, auto NV) {
+        diff_gkv_kernel<T, decltype(G)::value, decltype(NV)::value>
+            <<<(unsigned)blocks, 256, 0, st>>>(a);
+      });
+      return 0;
+    });
+    GATX_LAUNCH_CHECK("diff_attention_gkv");
+    if (a.w.hub_blocks) {
+      GATX_GRID(src_hub_bound * heads, "diff_attention_backward");
+      with_dtype(dtype, [&](auto t) {
+        using T = decltype(t);
+        diff_grad_join_kernel<T><<<(unsigned)(src_hub_bound * heads), 256, 0, st>>>(a, (T*)gk,
+                                                                                   (T*)gv);
+        return 0;
+      });
+      GATX_LAUNCH_CHECK("diff_attention_gkv_join");
+    }
+  }
+  return 0;
+}

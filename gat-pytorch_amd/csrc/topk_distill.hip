@@ -1,0 +1,496 @@
+// Distillation from a teacher's top logits: loss_i = T^2 sum_k p_k (log p_k - log q[c_k]) with
+// p = softmax over the row's K kept teacher logits of t / T and q = softmax over all classes of
+// s / T; d loss_i / d s_j = T (q_j - sum of the p_k with c_k = j).
+//
+// HBM-bound: the forward streams the logits once (a running maximum and sum a lane, joined at the
+// end), the backward streams them again and writes the gradient, from the two maxima and sums that
+// the forward kept (16 bytes a row) rather than a stored gradient of the size of the logits, which
+// would have to be scaled, and so read and written, once more. The gradient is written as g T q
+// first; the row's few taught classes are then written again by the same workgroup, the slots of
+// one class added in slot order, so the result does not depend on the order of anything.
+//
+// Rows of up to 1024 classes and 64 slots: a group of 8..64 lanes of a wave each, walking the rows
+// in a fixed stride. Wider rows: a workgroup each, 16-byte accesses from the first aligned element
+// on (rows of an odd number of classes start anywhere).
+#include "dtypes.h"
+
+namespace gatx {
+namespace {
+
+constexpr int kMaxSlots = 1024;
+constexpr int kGroupSlots = 64, kGroupClasses = 1024;
+constexpr int kMaxBlocks = 2048;
+constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
+constexpr float kInf = __builtin_huge_valf();
+
+struct DistillArgs {
+  const void *logits, *teacher, *index;
+  int64_t rows, ld;
+  int classes, K, teacher_dtype, index64, lanes;
+  float T, k;        // k = log2(e) / T
+  float* row_loss;
+  float* part;       // [blocks][2]: loss, rows with slots
+  float* stat;       // [rows][4]: max s, log2 sum, max t, log2 sum (the last -inf: no slots)
+  const float *g, *count;
+  int g_stride;
+  void* grad;
+};
+
+__device__ inline float teacher_at(const DistillArgs& a, int64_t i) {
+  if (a.teacher_dtype == GATX_F32) return ((const float*)a.teacher)[i];
+  if (a.teacher_dtype == GATX_BF16) return (float)((const __bf16*)a.teacher)[i];
+  return (float)((const _Float16*)a.teacher)[i];
+}
+// The slot's class; -1: empty. Classes past the last one stay what they are (as INT_MAX).
+__device__ inline int class_at(const DistillArgs& a, int64_t i) {
+  const int64_t c = a.index64 ? ((const int64_t*)a.index)[i] : ((const int32_t*)a.index)[i];
+  return c < 0 ? -1 : c >= a.classes ? 0x7fffffff : (int)c;
+}
+
+// Running maximum and sum of exp2((x - m) k).
+struct Lse {
+  float m = -kInf, s = 0.f;
+};
+template <int N>
+__device__ inline void lse_add(Lse& z, const float (&x)[N], float k) {
+  float mx = x[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i) mx = fmaxf(mx, x[i]);
+  mx = fmaxf(mx, z.m);
+  const float ref = mx == -kInf ? 0.f : mx;   // nothing but -inf so far: every term is 0
+  float s = z.s * __builtin_amdgcn_exp2f((z.m - ref) * k);
+#pragma unroll
+  for (int i = 0; i < N; ++i) s += __builtin_amdgcn_exp2f((x[i] - ref) * k);
+  z.m = mx;
+  z.s = s;
+}
+__device__ inline void lse_join(Lse& z, float m, float s, float k) {
+  const float mx = fmaxf(z.m, m), ref = mx == -kInf ? 0.f : mx;
+  z.s = z.s * __builtin_amdgcn_exp2f((z.m - ref) * k) + s * __builtin_amdgcn_exp2f((m - ref) * k);
+  z.m = mx;
+}
+__device__ inline void lse_join_lanes(Lse& z, int lanes, float k) {
+  for (int d = 1; d < lanes; d <<= 1) {
+    const float m = __shfl_xor(z.m, d), s = __shfl_xor(z.s, d);
+    // both partners add the same two terms in the same order
+    const bool low = !(threadIdx.x & d);
+    Lse lo{low ? z.m : m, low ? z.s : s};
+    lse_join(lo, low ? m : z.m, low ? s : z.s, k);
+    z = lo;
+  }
+}
+__device__ inline float lanes_total(float v, int lanes) {
+  for (int d = 1; d < lanes; d <<= 1) v += __shfl_xor(v, d);
+  return v;
+}
+__device__ inline float lanes_most(float v, int lanes) {
+  for (int d = 1; d < lanes; d <<= 1) v = fmaxf(v, __shfl_xor(v, d));
+  return v;
+}
+
+// One row's teacher: a lane's slots li, li + lanes, ...: the largest logit and whether any counts.
+__device__ inline float teacher_max(const DistillArgs& a, int64_t at, int li, int lanes, bool& bad) {
+  float tm = -kInf;
+  bad = false;
+  for (int j = li; j < a.K; j += lanes) {
+    const int c = class_at(a, at + j);
+    if (c < 0) continue;
+    const float t = teacher_at(a, at + j);
+    if (t == -kInf) continue;
+    bad |= c == 0x7fffffff || t != t;
+    tm = fmaxf(tm, t);
+  }
+  return tm;
+}
+__device__ inline float teacher_sum(const DistillArgs& a, int64_t at, int li, int lanes, float tm) {
+  float ts = 0.f;
+  for (int j = li; j < a.K; j += lanes) {
+    if (class_at(a, at + j) < 0) continue;
+    const float t = teacher_at(a, at + j);
+    if (t != -kInf) ts += __builtin_amdgcn_exp2f((t - tm) * a.k);
+  }
+  return ts;
+}
+// Its share of sum_k p_k (log p_k - log q[c_k]), in units of ln 2: the logarithms are base 2.
+template <typename T>
+__device__ inline float slots_loss(const DistillArgs& a, const T* row, int64_t at, int li,
+                                   int lanes, float m, float ls, float tm, float lts) {
+  float sum = 0.f;
+  for (int j = li; j < a.K; j += lanes) {
+    const int c = class_at(a, at + j);
+    if (c < 0 || c == 0x7fffffff) continue;
+    const float t = teacher_at(a, at + j);
+    if (t == -kInf) continue;
+    const float lp = (t - tm) * a.k - lts, p = __builtin_amdgcn_exp2f(lp);
+    if (p > 0.f) sum += p * (lp - (((float)row[c] - m) * a.k - ls));
+    else if (p != p) sum = p;
+  }
+  return sum;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) distill_group_kernel(DistillArgs a) {
+  __shared__ float red[2][32];
+  const int lanes = a.lanes, li = threadIdx.x & (lanes - 1), grp = threadIdx.x / lanes;
+  const int groups = 256 / lanes;
+  float total = 0.f, some = 0.f;
+  for (int64_t r0 = (int64_t)blockIdx.x * groups; r0 < a.rows; r0 += (int64_t)gridDim.x * groups) {
+    const int64_t r = r0 + grp;
+    if (r >= a.rows) continue;   // whole groups drop out; exchanges stay within a group
+    const T* row = (const T*)a.logits + r * a.ld;
+    const int64_t at = r * a.K;
+    Lse z;
+    for (int c = li; c < a.classes; c += 4 * lanes) {
+      float x[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) x[u] = c + u * lanes < a.classes ? (float)row[c + u * lanes] : -kInf;
+      lse_add(z, x, a.k);
+    }
+    lse_join_lanes(z, lanes, a.k);
+    bool bad;
+    float tm = teacher_max(a, at, li, lanes, bad);
+    tm = lanes_most(tm, lanes);
+    const bool any_bad = lanes_most(bad ? 1.f : 0.f, lanes) > 0.f;
+    const bool has = tm != -kInf || any_bad;
+    const float ts = lanes_total(teacher_sum(a, at, li, lanes, tm), lanes);
+    const float ls = __builtin_amdgcn_logf(z.s), lts = __builtin_amdgcn_logf(ts);
+    float loss = 0.f;
+    if (has) {
+      loss = lanes_total(slots_loss(a, row, at, li, lanes, z.m, ls, tm, lts), lanes);
+      loss = any_bad ? __builtin_nanf("") : loss * (a.T * a.T * kLn2);
+    }
+    if (li == 0) {
+      if (a.row_loss) a.row_loss[r] = loss;
+      if (a.stat)
+        *(float4*)(a.stat + 4 * r) = make_float4(z.m, ls, tm, lts);
+      total += loss;
+      some += has ? 1.f : 0.f;
+    }
+  }
+  if (!a.part) return;
+  if (li == 0) {
+    red[0][grp] = total;
+    red[1][grp] = some;
+  }
+  __syncthreads();
+  if (threadIdx.x < 2) {
+    float s = 0.f;
+    for (int i = 0; i < groups; ++i) s += red[threadIdx.x][i];
+    a.part[2 * blockIdx.x + threadIdx.x] = s;
+  }
+}
+
+// Elements of a row before its first 16-byte boundary.
+template <typename T>
+__device__ inline int unaligned_head(const T* p, int n) {
+  const int off = (int)(((uintptr_t)p & 15) / sizeof(T));
+  return min(n, off ? (int)(16 / sizeof(T)) - off : 0);
+}
+
+__device__ inline float block_total(float v, float* red) {
+  v = group_sum<64>(v);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  float s = 0.f;
+  for (int i = 0; i < (int)(blockDim.x >> 6); ++i) s += red[i];
+  return s;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(1024) distill_block_kernel(DistillArgs a) {
+  constexpr int V = 16 / sizeof(T);
+  __shared__ float red[16], red_m[16], red_s[16], red_t[16];
+  const int tid = threadIdx.x, nt = blockDim.x;
+  float total = 0.f, some = 0.f;
+  for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+    const T* row = (const T*)a.logits + r * a.ld;
+    const int64_t at = r * a.K;
+    const int head = unaligned_head(row, a.classes);
+    const int chunks = (a.classes - head) / V, tail = head + chunks * V;
+    Lse z;
+    {
+      float x[1] = {-kInf};
+      if (tid < head) x[0] = (float)row[tid];
+      else if (tid >= V && tid - V < a.classes - tail) x[0] = (float)row[tail + tid - V];
+      if (tid < 2 * V) lse_add(z, x, a.k);
+    }
+    const T* body = row + head;
+    int c = tid;
+    for (; c + nt < chunks; c += 2 * nt) {
+      float x[2 * V], y[V], w[V];
+      load_f32(body + (int64_t)c * V, y);
+      load_f32(body + (int64_t)(c + nt) * V, w);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        x[i] = y[i];
+        x[V + i] = w[i];
+      }
+      lse_add(z, x, a.k);
+    }
+    if (c < chunks) {
+      float x[V];
+      load_f32(body + (int64_t)c * V, x);
+      lse_add(z, x, a.k);
+    }
+    lse_join_lanes(z, 64, a.k);
+    bool bad;
+    float tm = lanes_most(teacher_max(a, at, tid, nt, bad), 64);
+    const float nbad = block_total(bad ? 1.f : 0.f, red);   // its barriers: the last
+                                                            // row's readers of red_m, red_s, red_t
+    if ((tid & 63) == 0) {
+      red_m[tid >> 6] = z.m;
+      red_s[tid >> 6] = z.s;
+      red_t[tid >> 6] = tm;
+    }
+    __syncthreads();
+    z = Lse{red_m[0], red_s[0]};
+    tm = red_t[0];
+    for (int i = 1; i < nt >> 6; ++i) {
+      lse_join(z, red_m[i], red_s[i], a.k);
+      tm = fmaxf(tm, red_t[i]);
+    }
+    const bool has = tm != -kInf || nbad > 0.f;
+    const float ts = block_total(teacher_sum(a, at, tid, nt, tm), red);
+    const float ls = __builtin_amdgcn_logf(z.s), lts = __builtin_amdgcn_logf(ts);
+    float loss = block_total(
+        has ? slots_loss(a, row, at, tid, nt, z.m, ls, tm, lts) : 0.f, red);
+    loss = nbad > 0.f ? __builtin_nanf("") : loss * (a.T * a.T * kLn2);
+    if (tid == 0) {
+      if (a.row_loss) a.row_loss[r] = loss;
+      if (a.stat)
+        *(float4*)(a.stat + 4 * r) = make_float4(z.m, ls, tm, lts);
+      total += loss;
+      some += has ? 1.f : 0.f;
+    }
+  }
+  if (tid == 0 && a.part) {
+    a.part[2 * blockIdx.x] = total;
+    a.part[2 * blockIdx.x + 1] = some;
+  }
+}
+
+__global__ void __launch_bounds__(1024) distill_total_kernel(const float* part, int blocks,
+                                                             float* total) {
+  __shared__ float red[16];
+  float l = 0.f, n = 0.f;
+  for (int i = threadIdx.x; i < blocks; i += 1024) {
+    l += part[2 * i];
+    n += part[2 * i + 1];
+  }
+  l = block_total(l, red);
+  n = block_total(n, red);
+  if (threadIdx.x == 0) {
+    total[0] = l;
+    total[1] = n;
+    total[2] = l / fmaxf(n, 1.f);
+  }
+}
+
+// The row's slots in LDS: class (-1: empty) and p. Returns whether a class is out of range.
+__device__ inline bool stage_slots(const DistillArgs& a, int64_t at, int li, int lanes, float tm,
+                                   float lts, int* cls, float* ps) {
+  bool bad = false;
+  for (int j = li; j < a.K; j += lanes) {
+    int c = class_at(a, at + j);
+    float p = 0.f;
+    if (c >= 0) {
+      const float t = teacher_at(a, at + j);
+      if (t == -kInf) c = -1;
+      else p = __builtin_amdgcn_exp2f((t - tm) * a.k - lts);
+      bad |= c == 0x7fffffff;
+    }
+    cls[j] = c == 0x7fffffff ? -1 : c;
+    ps[j] = p;
+  }
+  return bad;
+}
+// The taught classes' gradients: the first slot of a class adds up all of its slots.
+template <typename T>
+__device__ inline void write_slots(const DistillArgs& a, const T* row, T* grad, int li, int lanes,
+                                   float gi, float m, float ls, const int* cls, const float* ps) {
+  for (int j = li; j < a.K; j += lanes) {
+    const int c = cls[j];
+    if (c < 0) continue;
+    float p = 0.f;
+    bool first = true;
+    for (int i = 0; i < a.K; ++i)
+      if (cls[i] == c) {
+        p += ps[i];
+        first &= i >= j;
+      }
+    if (first) grad[c] = (T)(gi * (__builtin_amdgcn_exp2f(((float)row[c] - m) * a.k - ls) - p));
+  }
+}
+__device__ inline float row_factor(const DistillArgs& a, int64_t r) {
+  float gi = a.g[r * a.g_stride] * a.T;
+  if (a.count) gi /= fmaxf(*a.count, 1.f);
+  return gi;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) distill_group_grad_kernel(DistillArgs a) {
+  __shared__ int cls_lds[32 * kGroupSlots];
+  __shared__ float p_lds[32 * kGroupSlots];
+  const int lanes = a.lanes, li = threadIdx.x & (lanes - 1), grp = threadIdx.x / lanes;
+  const int groups = 256 / lanes;
+  int* cls = cls_lds + grp * kGroupSlots;
+  float* ps = p_lds + grp * kGroupSlots;
+  for (int64_t r0 = (int64_t)blockIdx.x * groups; r0 < a.rows; r0 += (int64_t)gridDim.x * groups) {
+    const int64_t r = r0 + grp;
+    if (r >= a.rows) continue;
+    const T* row = (const T*)a.logits + r * a.ld;
+    T* grad = (T*)a.grad + r * a.classes;
+    const float4 st = *(const float4*)(a.stat + 4 * r);
+    const bool has = st.w != -kInf;
+    float gi = row_factor(a, r);
+    bool bad = st.w != st.w;
+    if (has) bad |= stage_slots(a, r * a.K, li, lanes, st.z, st.w, cls, ps);
+    if (lanes_most(bad ? 1.f : 0.f, lanes) > 0.f) gi = __builtin_nanf("");
+    for (int c = li; c < a.classes; c += lanes)
+      grad[c] = (T)(has ? gi * __builtin_amdgcn_exp2f(((float)row[c] - st.x) * a.k - st.y) : 0.f);
+    wave_lds_sync();   // the slots and the stores above, before this wave's next ones
+    if (has) write_slots(a, row, grad, li, lanes, gi, st.x, st.y, cls, ps);
+    wave_lds_sync();
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(1024) distill_block_grad_kernel(DistillArgs a) {
+  constexpr int V = 16 / sizeof(T);
+  __shared__ int cls[kMaxSlots];
+  __shared__ float ps[kMaxSlots];
+  __shared__ float red[16];
+  const int tid = threadIdx.x, nt = blockDim.x;
+  for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+    const T* row = (const T*)a.logits + r * a.ld;
+    T* grad = (T*)a.grad + r * a.classes;
+    const float4 st = *(const float4*)(a.stat + 4 * r);
+    const bool has = st.w != -kInf;
+    float gi = row_factor(a, r);
+    __syncthreads();   // the last row's readers of the slots
+    bool bad = st.w != st.w;
+    if (has) bad |= stage_slots(a, r * a.K, tid, nt, st.z, st.w, cls, ps);
+    if (block_total(bad ? 1.f : 0.f, red) > 0.f) gi = __builtin_nanf("");
+    auto value = [&](float x) {
+      return has ? gi * __builtin_amdgcn_exp2f((x - st.x) * a.k - st.y) : 0.f;
+    };
+    const int head = unaligned_head(grad, a.classes);
+    if (head == unaligned_head(row, a.classes)) {
+      const int chunks = (a.classes - head) / V, tail = head + chunks * V;
+      if (tid < head) grad[tid] = (T)value((float)row[tid]);
+      if (tid < a.classes - tail) grad[tail + tid] = (T)value((float)row[tail + tid]);
+      for (int c = tid; c < chunks; c += nt) {
+        float x[V];
+        load_f32(row + head + (int64_t)c * V, x);
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[i] = value(x[i]);
+        store_f32(grad + head + (int64_t)c * V, x);
+      }
+    } else {   // rows of another alignment than the gradient's
+      for (int c = tid; c < a.classes; c += nt) grad[c] = (T)value((float)row[c]);
+    }
+    __syncthreads();   // every store above is before the taught classes' own
+    if (has) write_slots(a, row, grad, tid, nt, gi, st.x, st.y, cls, ps);
+  }
+}
+
+bool group_form(int64_t classes, int K) { return classes <= kGroupClasses && K <= kGroupSlots; }
+int group_lanes(int64_t classes) {
+  int l = 8;
+  while (l < 64 && l * 4 < classes) l <<= 1;
+  return l;
+}
+int distill_blocks(int64_t rows, int64_t classes, int K) {
+  const int64_t per = group_form(classes, K) ? 256 / group_lanes(classes) : 1;
+  return (int)std::min<int64_t>(ceil_div(rows, per), kMaxBlocks);
+}
+// A workgroup a row: few rows leave CUs to themselves, so each gets all the lanes it can have
+int block_threads(int64_t rows) { return rows >= 512 ? 256 : 1024; }
+
+int check_distill(const char* what, int dtype, int64_t rows, int64_t classes, int teacher_dtype,
+                  int K, float temperature) {
+  GATX_REQUIRE(dtype_ok(dtype) && dtype_ok(teacher_dtype), "%s: unknown dtype", what);
+  GATX_REQUIRE(rows >= 0 && classes >= 1 && classes < (1ll << 30), "%s: %lld x %lld logits", what,
+               (long long)rows, (long long)classes);
+  GATX_REQUIRE(K >= 1 && K <= kMaxSlots, "%s: %d slots a row (1..%d)", what, K, kMaxSlots);
+  GATX_REQUIRE(temperature > 0.f && temperature < kInf, "%s: temperature must be positive", what);
+  return 0;
+}
+
+}  // namespace
+}  // namespace gatx
+
+using namespace gatx;
+
+extern "C" size_t gatx_topk_distill_workspace_bytes(int64_t rows) {
+  return sizeof(float) * 2 * (size_t)std::min<int64_t>(std::max<int64_t>(rows, 1), kMaxBlocks);
+}
+
+extern "C" int gatx_topk_distill(int dtype, const void* logits, int64_t rows, int64_t classes,
+                                 int64_t ld, int teacher_dtype, const void* teacher,
+                                 const void* index, int index_is_int64, int K, float temperature,
+                                 float* row_loss, float* total, float* stat, void* workspace,
+                                 size_t workspace_bytes, gatx_stream_t s) {
+  GATX_CALL(check_distill("topk_distill", dtype, rows, classes, teacher_dtype, K, temperature));
+  hipStream_t st = (hipStream_t)s;
+  if (rows == 0) {
+    if (total) zero_words_kernel<<<1, 64, 0, st>>>((uint32_t*)total, 3);
+    GATX_LAUNCH_CHECK("topk_distill zero");
+    return 0;
+  }
+  GATX_REQUIRE(logits && teacher && index, "topk_distill: null input");
+  GATX_REQUIRE(!total || (workspace && workspace_bytes >= gatx_topk_distill_workspace_bytes(rows)),
+               "topk_distill: workspace too small");
+  DistillArgs a = {};
+  a.logits = logits; a.teacher = teacher; a.index = index; a.rows = rows; a.ld = ld;
+  a.classes = (int)classes; a.K = K; a.teacher_dtype = teacher_dtype; a.index64 = index_is_int64;
+  a.T = temperature; a.k = kLog2e / temperature;
+  a.row_loss = row_loss; a.part = total ? (float*)workspace : nullptr; a.stat = stat;
+  a.lanes = group_lanes(classes);
+  const int blocks = distill_blocks(rows, classes, K);
+  with_dtype(dtype, [&](auto t) {
+    using T = decltype(t);
+    if (group_form(classes, K)) distill_group_kernel<T><<<blocks, 256, 0, st>>>(a);
+    else distill_block_kernel<T><<<blocks, block_threads(rows), 0, st>>>(a);
+    return 0;
+  });
+  GATX_LAUNCH_CHECK("topk_distill");
+  if (total) {
+    distill_total_kernel<<<1, 1024, 0, st>>>((const float*)workspace, blocks, total);
+    GATX_LAUNCH_CHECK("topk_distill_total");
+  }
+  return 0;
+}
+
+extern "C" int gatx_topk_distill_backward(int dtype, const void* logits, int64_t rows,
+                                          int64_t classes, int64_t ld, int teacher_dtype,
+                                          const void* teacher, const void* index,
+                                          int index_is_int64, int K, float temperature,
+                                          const float* stat, const float* g, int g_stride,
+                                          const float* count, void* grad, gatx_stream_t s) {
+  GATX_CALL(check_distill("topk_distill_backward", dtype, rows, classes, teacher_dtype, K,
+                          temperature));
+  if (rows == 0) return 0;
+  GATX_REQUIRE(logits && teacher && index && stat && g && grad,
+               "topk_distill_backward: null buffer");
+  GATX_REQUIRE(g_stride == 0 || g_stride == 1, "topk_distill_backward: g_stride is 0 or 1");
+  DistillArgs a = {};
+  a.logits = logits; a.teacher = teacher; a.index = index; a.rows = rows; a.ld = ld;
+  a.classes = (int)classes; a.K = K; a.teacher_dtype = teacher_dtype; a.index64 = index_is_int64;
+  a.T = temperature; a.k = kLog2e / temperature;
+  a.stat = const_cast<float*>(stat); a.g = g; a.count = count; a.g_stride = g_stride;
+  a.grad = grad; a.lanes = group_lanes(classes);
+  hipStream_t st = (hipStream_t)s;
+  // every row's work is its own: as many workgroups as rows fill, no fixed walk to keep
+  const int64_t per = group_form(classes, K) ? 256 / a.lanes : 1;
+  const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(rows, per), 1 << 20);
+  with_dtype(dtype, [&](auto t) {
+    using T = decltype(t);
+    if (group_form(classes, K)) distill_group_grad_kernel<T><<<blocks, 256, 0, st>>>(a);
+    else distill_block_grad_kernel<T><<<blocks, block_threads(rows), 0, st>>>(a);
+    return 0;
+  });
+  GATX_LAUNCH_CHECK("topk_distill_backward");
+  return 0;
+}

@@ -2,6 +2,8 @@
 
     from gatx import GATLayer          # == models/gat_layer.py:GATLayer, on libgatx.so (HIP)
     from gatx import GATModel          # layer stack wiring of models/GATModel.py (no Lightning)
+    from gatx import DiffAttention     # differential attention on the same graphs (gatx.attention)
+    from gatx import BlockNorm         # the norms around a block, gate and residual (gatx.norms)
 
 Submodules `gatx.data`, `gatx.config`, `gatx.checkpoint`, `gatx.tuning` (the host path's explicit
 switches; nothing is read from the environment) are pure Python/numpy. Everything that
@@ -16,6 +18,11 @@ _LAZY = {
     "Graph": ("graph", "Graph"),
     "clear_graph_cache": ("graph", "clear_graph_cache"),
     "gat_layer": ("functional", "gat_layer"),
+    "diff_attention": ("attention", "diff_attention"),
+    "DiffAttention": ("attention", "DiffAttention"),
+    "norm_before": ("norms", "norm_before"),
+    "norm_after": ("norms", "norm_after"),
+    "BlockNorm": ("norms", "BlockNorm"),
 }
 
 

@@ -139,6 +139,30 @@ SIGNATURES = {
     "gatx_attention_norm_backward": (c_i, [P, c_i64, c_i, P, c_i, P, P, c_f, P, P]),
     "gatx_attention_norm_multi_workspace_bytes": (c_sz, [c_i]),
     "gatx_attention_norm_multi": (c_i, [P, P, c_i, c_i64, P, c_i, P, c_f, P, P, P]),
+    "gatx_relative_buckets": (c_i, [P, P, P, c_i64, c_i64, P, c_i64, P, c_i, c_i, P, c_i, c_i, P,
+                                    P]),
+    "gatx_diff_attention_pack": (c_i, [c_i, c_i64, c_i64, c_i, c_i, c_i, P, c_i64, P, P, c_i64, P,
+                                       P, c_i64, P, P]),
+    "gatx_diff_attention_part_bytes": (c_sz, [c_i64, c_i, c_i]),
+    "gatx_diff_attention": (c_i, [c_i, P, c_i64, P, c_i64, P, c_i64, c_i, c_i, c_i, P, P, c_i64,
+                                  c_i64, c_i64, P, c_i, c_f, P, P, P, P, P, P, c_i, P, P, c_i64,
+                                  P, c_sz, P]),
+    "gatx_diff_attention_backward_workspace_bytes": (c_sz, [c_i64, c_i64, c_i, c_i, c_i, c_i,
+                                                            c_i64, c_i64]),
+    "gatx_diff_attention_backward": (c_i, [c_i, P, c_i64, P, c_i64, P, c_i64, P, c_i64, c_i, c_i,
+                                           c_i, P, P, P, P, P, c_i64, c_i64, c_f, P, P, c_i, P, P,
+                                           P, P, P, P, P, c_i, P, P, c_i64, P, P, c_i64, P, c_sz,
+                                           P]),
+    "gatx_block_norm": (c_i, [c_i, c_i64, c_i64, P, c_i64, P, P, c_i64, P, c_i, c_i64, P, P, c_f,
+                              P, P, P, P, P]),
+    "gatx_block_norm_backward_workspace_bytes": (c_sz, [c_i64, c_i64]),
+    "gatx_block_norm_backward": (c_i, [c_i, c_i64, c_i64, P, c_i64, P, P, c_i64, P, c_i, c_i64, P,
+                                       P, P, P, P, c_i64, P, c_i64, P, P, P, P, P, P, P, c_sz, P]),
+    "gatx_topk_distill_workspace_bytes": (c_sz, [c_i64]),
+    "gatx_topk_distill": (c_i, [c_i, P, c_i64, c_i64, c_i64, c_i, P, P, c_i, c_i, c_f, P, P, P, P,
+                                c_sz, P]),
+    "gatx_topk_distill_backward": (c_i, [c_i, P, c_i64, c_i64, c_i64, c_i, P, P, c_i, c_i, c_f, P,
+                                         P, c_i, P, P, P]),
 }
 
 
@@ -179,6 +203,9 @@ def version(t) -> int:
     """In-place version counter of a tensor for cache keys. Inference tensors (made under
     torch.inference_mode) track none and cannot be modified in place outside it: 0."""
     return 0 if t.is_inference() else t._version
+
+
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # GATX_F32, GATX_BF16, GATX_F16
 
 
 def stream() -> int:

@@ -2,12 +2,15 @@
 reduction and an optional scalar pos_weight — PPI_GAT's `nn.BCEWithLogitsLoss()`
 (`models/ppi_gat.py:11,19`) and PatternGAT's `nn.BCEWithLogitsLoss(pos_weight=1/0.1765)`
 (`models/pattern_gat.py:11-15`). One launch computes the loss and its gradient; the backward is
-one scaling launch (torch: ~19 launches for forward + backward)."""
+one scaling launch (torch: ~19 launches for forward + backward).
+
+And distillation from a teacher's top logits (csrc/topk_distill.hip)."""
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
-from ._lib import call, lib, ptr, stream
+from ._lib import DTYPES, call, lib, ptr, stream
 from .functional import _span
 
 
@@ -80,3 +83,107 @@ class BCEWithLogitsLoss(torch.nn.Module):
 
     def forward(self, input, target):
         return BCEWithLogitsFunction.apply(input, target, self.pw)
+
+
+class TopKDistillationFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, teacher, index, temperature: float, reduction: str):
+        dev = logits.device
+        n, C = logits.shape
+        K = teacher.size(1)
+        x = logits
+        if C > 1 and x.stride(1) != 1:
+            x = x.contiguous()
+        ld = x.stride(0) if n > 1 else C
+        teacher, index = teacher.contiguous(), index.contiguous()
+        save = ctx.needs_input_grad[0]
+        none = reduction == "none"
+        row_loss = torch.empty(n, device=dev) if none else None
+        total = None if none else torch.empty(3, device=dev)
+        stat = torch.empty((n, 4), device=dev) if save else None
+        wb = 0 if none else lib.gatx_topk_distill_workspace_bytes(n)
+        ws = torch.empty(wb, dtype=torch.uint8, device=dev) if wb else None
+        args = (DTYPES[x.dtype], ptr(x), n, C, ld, DTYPES[teacher.dtype], ptr(teacher),
+                ptr(index), int(index.dtype == torch.int64), K, temperature)
+        with _span("topk_distill", (n, C, K)):
+            call("gatx_topk_distill", *args, ptr(row_loss), ptr(total), ptr(stat), ptr(ws), wb,
+                 stream())
+        if save:
+            ctx.save_for_backward(x, teacher, index, stat, total)
+            ctx.args, ctx.reduction = (ld, temperature), reduction
+        return row_loss if none else total[2] if reduction == "mean" else total[0]
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        x, teacher, index, stat, total = ctx.saved_tensors
+        (ld, temperature), (n, C) = ctx.args, x.shape
+        with torch.cuda.device(x.device):
+            g = g.to(torch.float32).contiguous()
+            grad = torch.empty((n, C), dtype=x.dtype, device=x.device)
+            count = ptr(total) + 4 if ctx.reduction == "mean" else None
+            with _span("topk_distill_bwd", (n, C)):
+                call("gatx_topk_distill_backward", DTYPES[x.dtype], ptr(x), n, C, ld,
+                     DTYPES[teacher.dtype], ptr(teacher), ptr(index),
+                     int(index.dtype == torch.int64), teacher.size(1), temperature, ptr(stat),
+                     ptr(g), int(ctx.reduction == "none"), count, ptr(grad), stream())
+        return grad, None, None, None, None
+
+
+def topk_distillation(logits: torch.Tensor, teacher_logits: torch.Tensor,
+                      teacher_index: torch.Tensor, temperature: float = 1.0,
+                      reduction: str = "mean") -> torch.Tensor:
+    """Distillation from the K logits that were kept of a teacher's: T^2 KL(p || q) per row, p the
+    softmax of teacher_logits / T over the row's slots, q that of logits / T over all classes.
+
+    logits (rows, classes), teacher_logits (rows, K) (each float32, bfloat16 or float16),
+    teacher_index (rows, K) int64 or int32: the slots' classes, K <= 1024. A negative class (or a
+    teacher logit of -inf) is an empty slot; a class may come twice; one past the last makes its
+    row NaN. A row without slots has loss 0 and no gradient. reduction "mean" is over the rows that
+    have slots (0 if none has), "sum", or "none" (one float32 a row). Only logits get a gradient."""
+    for name, t in (("logits", logits), ("teacher_logits", teacher_logits),
+                    ("teacher_index", teacher_index)):
+        if t.device != logits.device:
+            raise RuntimeError(f"gatx: topk_distillation: {name} is on {t.device}, logits on "
+                               f"{logits.device}")
+        if t.dim() != 2:
+            raise ValueError(f"gatx: topk_distillation: {name} has two dimensions, got "
+                             f"{tuple(t.shape)}")
+    if logits.dtype not in DTYPES or teacher_logits.dtype not in DTYPES:
+        raise RuntimeError("gatx: topk_distillation takes float32, bfloat16 or float16 logits, got "
+                           f"{logits.dtype} and {teacher_logits.dtype}")
+    if teacher_index.dtype not in (torch.int64, torch.int32):
+        raise RuntimeError("gatx: topk_distillation: teacher_index must be int64 or int32, got "
+                           f"{teacher_index.dtype}")
+    if (teacher_logits.shape != teacher_index.shape or logits.size(0) != teacher_index.size(0)
+            or logits.size(1) < 1 or not 1 <= teacher_index.size(1) <= 1024):
+        raise ValueError("gatx: topk_distillation: (rows, classes) logits and (rows, K <= 1024) "
+                         f"teacher logits and classes, got {tuple(logits.shape)}, "
+                         f"{tuple(teacher_logits.shape)}, {tuple(teacher_index.shape)}")
+    if teacher_logits.requires_grad:
+        raise RuntimeError("gatx: topk_distillation does not differentiate the teacher; pass "
+                           "teacher_logits.detach()")
+    temperature = float(temperature)
+    if not 0.0 < temperature < float("inf"):
+        raise ValueError(f"gatx: topk_distillation: temperature must be positive, got "
+                         f"{temperature}")
+    if reduction not in ("mean", "sum", "none"):
+        raise ValueError(f"gatx: topk_distillation: reduction {reduction!r} is not mean, sum or "
+                         "none")
+    if not logits.is_cuda:
+        raise RuntimeError("gatx: topk_distillation needs HIP tensors (no CPU path)")
+    with torch.cuda.device(logits.device):
+        return TopKDistillationFunction.apply(logits, teacher_logits, teacher_index, temperature,
+                                              reduction)
+
+
+class TopKDistillationLoss(torch.nn.Module):
+    """topk_distillation as a module (temperature and reduction fixed at construction)."""
+
+    def __init__(self, temperature: float = 1.0, reduction: str = "mean"):
+        super().__init__()
+        self.temperature, self.reduction = temperature, reduction
+
+    def forward(self, logits, teacher_logits, teacher_index):
+        return topk_distillation(logits, teacher_logits, teacher_index, self.temperature,
+                                 self.reduction)

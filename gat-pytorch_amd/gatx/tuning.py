@@ -34,6 +34,8 @@ threshold of one); the defaults are the measured-best choices (§
   lds_min_edges   2^18  edge_lds / side_stream only on graphs of at least this many edges
                         (edge_index' bound): below it a step is launch-bound, and the extra
                         launches and cross-queue joins cost more than they save (PATTERN G=8)
+  attn_hub_edges  512   gatx.attention: rows (in the backward also source rows) of more edges than
+                        this run in pieces (0: never)
 
     import gatx
     with gatx.tuning.override(edge_chunk=2245):   # or gatx.tuning.set(...) / reset()
@@ -61,6 +63,7 @@ DEFAULTS = {
     "edge_lds_bwd": 1,
     "side_stream": 0,
     "lds_min_edges": 1 << 18,
+    "attn_hub_edges": 512,
 }
 
 _current = dict(DEFAULTS)

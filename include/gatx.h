@@ -608,6 +608,122 @@ int gatx_bce_logits(const float* x, const float* y, int64_t n, float pos_weight,
 int gatx_scale_by_scalar(const float* g, const float* v, int64_t n, float* out,
                          gatx_stream_t stream);
 
+/* ================================================================ graph-transformer operators
+ * Neighbourhood attention by the difference of two softmax maps, its relative position bias, the
+ * norms around a block and distillation from top logits. None of them is on the reference's path;
+ * they run on the same graphs (gatx_graph_build's CSR) beside its layers. Tensors of `dtype`
+ * (below) keep every sum, softmax statistic and gradient in fp32 and are rounded once, where a
+ * result is stored. */
+#define GATX_F32 0
+#define GATX_BF16 1
+#define GATX_F16 2
+
+/* Buckets of the relative position pos[col[e]] - pos[rowidx[e]] of every CSR slot e, bucket[e] < 256:
+ * `exact` distances of one bucket each, then bucket exact + j from the distance bounds[j - 1] on
+ * (host array of n_bounds ascending int64), `per_side` = exact + n_bounds + 1 > n_bounds in all;
+ * bidirectional: sources behind their destination (a position above its own) take the buckets from
+ * per_side on, else they all have distance 0. num_nodes rows; nodes (nullable, n_nodes int64): only
+ * the slots of these rows are written (ids outside [0, num_nodes) are skipped). */
+int gatx_relative_buckets(const int32_t* rowptr, const int32_t* col, const int32_t* rowidx,
+                          int64_t E, int64_t num_nodes, const int64_t* nodes, int64_t n_nodes,
+                          const void* pos, int pos_is64, int exact, const int64_t* bounds,
+                          int n_bounds, int bidirectional, uint8_t* bucket, gatx_stream_t stream);
+
+/* The attention's kernels read rows of whole 8-element chunks: head widths dp = round_up(d, 8) and
+ * dvp = round_up(dv, 8), 16-byte aligned rows. This copies what is not laid out so into packed rows
+ * (zero tails), one launch: q (rows x 2H groups of d), k (keys x 2H of d), v (keys x H of dv); a
+ * NULL source is skipped. Row strides ld* in elements. */
+int gatx_diff_attention_pack(int dtype, int64_t rows, int64_t keys, int num_heads, int d, int dv,
+                             const void* q, int64_t ldq, void* qp, const void* k, int64_t ldk,
+                             void* kp, const void* v, int64_t ldv, void* vp,
+                             gatx_stream_t stream);
+
+/* out[i,h] = sum over i's in-edges e of (p1[e,h] - lam[h] p2[e,h]) v[col[e],h], p_m = softmax over
+ * them of scale q[i,h,m] . k[col[e],h,m] + bias[bucket[e],h] (bias NULL: none; an entry of -inf
+ * shuts its bucket, whatever lies in the keys and values behind it). q: rows x (H,2,dp), k: keys x
+ * (H,2,dp), v: keys x (H,dvp), chunked as above (zero tails), row strides ld*; out: rows x (H,dv),
+ * packed, of `dtype`. A row without open edges gives zeros. d <= 256, dv <= 512.
+ * nodes (nullable): q row r is node nodes[r]'s (its CSR row; keys = num_nodes), each row's edges
+ * dealt to `pieces` >= 1 parallel pieces; an id outside [0, num_nodes) gives a row of NaN.
+ * nodes == NULL: rows == num_nodes; rows of more than hub_edges edges run in pieces (a plan of
+ * gatx_graph_hub_plan at hub_edges; hub_edges = 0: never).
+ * For the backward (both or neither): S (H x E x 2 logits) and stat (H x rows x {max1, 1/sum1, max2,
+ * 1/sum2}). part: gatx_diff_attention_part_bytes(). */
+size_t gatx_diff_attention_part_bytes(int64_t slots, int num_heads, int dvp);
+int gatx_diff_attention(int dtype, const void* q, int64_t ldq, const void* k, int64_t ldk,
+                        const void* v, int64_t ldv, int num_heads, int d, int dv,
+                        const int32_t* rowptr, const int32_t* col, int64_t E, int64_t rows,
+                        int64_t num_nodes, const int64_t* nodes, int pieces, float scale,
+                        const float* lam, const float* bias, const uint8_t* bucket, void* out,
+                        float* S, float* stat, int hub_edges, const int32_t* hubs,
+                        const int32_t* hub_count, int64_t hub_bound, void* part,
+                        size_t part_bytes, gatx_stream_t stream);
+/* Its gradients from go (num_nodes x (H,dvp), as v): gq, gk (num_nodes x (H,2,d)), gv
+ * (num_nodes x (H,dv)), glam (H), gbias (n_buckets x H); each nullable. S and stat are the
+ * forward's; srowptr / scol / seid the transposed CSR, with its own hub plan. Fixed-order sums.
+ * workspace: gatx_diff_attention_backward_workspace_bytes(). */
+size_t gatx_diff_attention_backward_workspace_bytes(int64_t num_nodes, int64_t E, int num_heads,
+                                                    int d, int dv, int n_buckets,
+                                                    int64_t hub_bound, int64_t src_hub_bound);
+int gatx_diff_attention_backward(int dtype, const void* q, int64_t ldq, const void* k, int64_t ldk,
+                                 const void* v, int64_t ldv, const void* go, int64_t ldgo,
+                                 int num_heads, int d, int dv, const int32_t* rowptr,
+                                 const int32_t* col, const int32_t* srowptr, const int32_t* scol,
+                                 const int32_t* seid, int64_t E, int64_t num_nodes, float scale,
+                                 const float* lam, const uint8_t* bucket, int n_buckets,
+                                 const float* S, const float* stat, void* gq, void* gk, void* gv,
+                                 float* glam, float* gbias, int hub_edges, const int32_t* hubs,
+                                 const int32_t* hub_count, int64_t hub_bound,
+                                 const int32_t* src_hubs, const int32_t* src_hub_count,
+                                 int64_t src_hub_bound, void* workspace, size_t workspace_bytes,
+                                 gatx_stream_t stream);
+
+/* The norms around a block, rows x cols (cols <= 8192), one pass: with rms(z) = z / sqrt(mean z^2 +
+ * eps), y = resid + scale * sigmoid(gate) * weight * rms(h) and next = next_weight * rms(y). weight,
+ * scale, next_weight: cols floats. Nullable: resid (0), gate (its factor is 1; gate_rows = 1: rows x
+ * cols of dtype, 0: cols floats), scale (1), next_weight with next. weight == NULL: y = h (the norm
+ * before a block alone; resid, gate, scale and y must be NULL). Row strides ld*; y and next packed,
+ * of dtype; y is rounded where it is stored, not where next reads it. rstd_h / rstd_y (nullable,
+ * rows floats): 1 / sqrt(...) of both norms, for the backward. */
+int gatx_block_norm(int dtype, int64_t rows, int64_t cols, const void* h, int64_t ldh,
+                    const float* weight, const void* resid, int64_t ldr, const void* gate,
+                    int gate_rows, int64_t ldg, const float* scale, const float* next_weight,
+                    float eps, void* y, void* next, float* rstd_h, float* rstd_y,
+                    gatx_stream_t stream);
+/* Gradients from gy and gn (of y and next; either nullable): gh, gresid, ggate (cols floats when
+ * gate_rows = 0), gweight, gscale, gnext (cols floats); each nullable. Fixed-order sums over the rows
+ * in the workspace (gatx_block_norm_backward_workspace_bytes). */
+size_t gatx_block_norm_backward_workspace_bytes(int64_t rows, int64_t cols);
+int gatx_block_norm_backward(int dtype, int64_t rows, int64_t cols, const void* h, int64_t ldh,
+                             const float* weight, const void* resid, int64_t ldr,
+                             const void* gate, int gate_rows, int64_t ldg, const float* scale,
+                             const float* next_weight, const float* rstd_h, const float* rstd_y,
+                             const void* gy, int64_t ldgy, const void* gn, int64_t ldgn, void* gh,
+                             void* gresid, void* ggate, float* gweight, float* gscale,
+                             float* gnext, void* workspace, size_t workspace_bytes,
+                             gatx_stream_t stream);
+
+/* Distillation from a teacher's top logits. Row i of logits s (rows x classes, row stride ld, dtype)
+ * against teacher t (rows x K, packed, teacher_dtype) at the classes index (rows x K, packed, int64
+ * or int32; a slot of a negative class or of teacher -inf is empty): p = softmax over the row's
+ * slots of t / T, q = softmax of s / T, loss_i = T^2 sum_k p_k (log p_k - log q[index_k]). A class
+ * may come twice (its slots add up). A row without slots has loss 0 and no gradient; an index >=
+ * classes makes its row NaN. row_loss (nullable): rows floats; total (nullable): {sum of the losses,
+ * the number of rows with slots, sum / max(number, 1)}. stat (rows x 4, nullable, for the
+ * backward): the maxima and the sums' logarithms (base 2) of both softmaxes. K <= 1024. workspace: gatx_topk_distill_workspace_bytes(). Fixed-order sums. */
+size_t gatx_topk_distill_workspace_bytes(int64_t rows);
+int gatx_topk_distill(int dtype, const void* logits, int64_t rows, int64_t classes, int64_t ld,
+                      int teacher_dtype, const void* teacher, const void* index,
+                      int index_is_int64, int K, float temperature, float* row_loss, float* total,
+                      float* stat, void* workspace, size_t workspace_bytes, gatx_stream_t stream);
+/* grad (rows x classes, packed, dtype) = g T (q - sum of p at each class), g = g[i * g_stride]
+ * (g_stride 0 or 1) divided by max(*count, 1) when count is given (the forward's &total[1]). */
+int gatx_topk_distill_backward(int dtype, const void* logits, int64_t rows, int64_t classes,
+                               int64_t ld, int teacher_dtype, const void* teacher,
+                               const void* index, int index_is_int64, int K, float temperature,
+                               const float* stat, const float* g, int g_stride, const float* count,
+                               void* grad, gatx_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
