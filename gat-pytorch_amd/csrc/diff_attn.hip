@@ -11,23 +11,28 @@
 // per head, from L2 as long as one head's rows of the nodes in flight fit there. So a work item is
 // (row, head), items run in chunks of kChunk rows one head after the other, and whole (chunk, head)
 // units go to one XCD. The products are sparse (a row's neighbours are shared with no other row),
-// so they run on the vector units: packed dot products for the 16-bit types, and sums in fp32.
+// so they run on the vector units, packed dot products for bf16, every sum in fp32.
 //
-// G lanes hold one edge: lane c of them the c-th 8-element chunk of both maps' keys and the chunks
-// c (and c + G) of the values, so a logit is one exchange over G lanes and nothing else crosses
-// lanes. 64 / G edges are in flight per wave ("slots"), `rows_per_wave` rows share the wave where
-// their degree would leave slots idle. Each slot keeps its own running maxima and sums over its
-// edges (one pass over the data), joined when the row ends. Rows of more than hub_edges edges, and
-// the few rows of a serving call, are cut into pieces with partial results, joined in piece order.
-// The backward is three gathers: dw and D over the values (A), gq over the keys (B, which also
-// leaves {scale dx_1, scale dx_2, w} of each edge), gk and gv over the queries and go by the
-// transposed CSR (C). Every sum has a fixed order.
+// G lanes hold one edge's row: lane c of them the c-th 8-element chunk (of both maps; chunks c and c
+// + G of the values). What an edge needs once (its index, logits, weights) is held by one lane
+// each, NL = min(G, 16) edges at a time, and handed to the G lanes by a broadcast within their 16
+// lanes; a tile's dot products are summed over the lanes by a reduce-scatter that leaves edge i's
+// with lane i. So every step but the multiply-adds over a row costs 1 / NL of an instruction per
+// edge and lane. 64 / G edges are in flight per wave; a row has gs = 16, 32 or 64 lanes (gs / G slots
+// of edges side by side, joined at its end).
+// Forward: the logits and each row's statistics (gathers k), then the weighted values (gathers v).
+// Backward: A: dw and D (v); B: gq, and {scale dx_1, scale dx_2, w} of each edge (k); C: gk and gv by
+// the transposed CSR (q and go). One gather a pass keeps a head's gathered rows of a graph inside
+// L2, and the sums of pieces (rows of more than hub_edges edges) are plain. A serving call takes
+// one kernel with a running softmax instead: its rows are cut into pieces whose partial results
+// carry their maxima, and it needs no array of logits. Every sum has a fixed order.
 #include "dtypes.h"
 
 namespace gatx {
 namespace {
 
 constexpr int kChunk = 2048;       // rows of a (chunk, head) unit
+constexpr int kWantWaves = 4096;   // 4 a SIMD
 constexpr int kMaxD = 256, kMaxDv = 512, kMaxBuckets = 256;
 constexpr float kInf = __builtin_huge_valf();
 constexpr float kLog2e = 1.44269504088896341f;
@@ -86,9 +91,12 @@ __device__ inline float dot2(__bf16, uint32_t a, uint32_t b, float c) {
   return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, a),
                                          __builtin_bit_cast(bf16x2, b), c, false);
 }
+// fp16: two mixed-precision multiply-adds, each rounded once. The packed fp16 dot product is less
+// exact: a sum of D_2 over 44 900 rows came out 1e-6 to 1e-5 off, against 1e-7 this way (and with
+// bf16's packed product).
 __device__ inline float dot2(_Float16, uint32_t a, uint32_t b, float c) {
-  return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, a), __builtin_bit_cast(f16x2, b), c,
-                                false);
+  const f16x2 x = __builtin_bit_cast(f16x2, a), y = __builtin_bit_cast(f16x2, b);
+  return fmaf((float)x.y, (float)y.y, fmaf((float)x.x, (float)y.x, c));
 }
 template <typename T>
 __device__ inline float dot8(const Raw<T>& a, const Raw<T>& b, float c) {
@@ -163,23 +171,33 @@ template <int G>
 __device__ inline float edge_sum(float v) {
   return group_sum<G>(v);
 }
-// Sum over the slots of a row (lanes l, l + G, ... of its GS), in every lane. Rotations inside 16
-// lanes, swaps beyond; GS >= 16.
-template <int G>
-__device__ inline float slots_sum(float v, int gs) {
-  if (G <= 8) v += dpp<0x128>(v);   // row_ror:8
-  if (G <= 4) v += dpp<0x124>(v);
-  if (G <= 2) v += dpp<0x122>(v);
-  if (G <= 1) v += dpp<0x121>(v);
+// Sums over the slots of a row (lanes l, l + G, ... of its gs >= 16), in every lane: rotations inside
+// 16 lanes, swaps beyond.
+template <int G, int N>
+__device__ inline void slots_sum(float (&v)[N], int gs) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (G <= 8) v[i] += dpp<0x128>(v[i]);   // row_ror:8
+    if (G <= 4) v[i] += dpp<0x124>(v[i]);
+    if (G <= 2) v[i] += dpp<0x122>(v[i]);
+    if (G <= 1) v[i] += dpp<0x121>(v[i]);
+  }
   if (G <= 16 && gs >= 32) {
-    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[i]), __float_as_uint(v[i]), false,
+                                                false);
+      v[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
   }
   if (gs >= 64) {
-    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[i]), __float_as_uint(v[i]), false,
+                                                false);
+      v[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
   }
-  return v;
 }
 template <int G>
 __device__ inline float slots_max(float v, int gs) {
@@ -193,75 +211,137 @@ __device__ inline int wave_max(int v) {
 }
 __device__ inline float exp_(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
 
+// Edges per tile and slot: one for each lane of an edge, 16 at most (what a DPP row spans).
+template <int G>
+constexpr int kTile = G < 16 ? G : 16;
+// x of the lane that holds edge I of the own slot's tile.
+template <int G, int I>
+__device__ inline int tile_get(int x) {
+  if constexpr (G >= 16) {
+    return __builtin_amdgcn_update_dpp(x, x, 0x150 + I, 0xf, 0xf, false);   // row_newbcast:I
+  } else if constexpr (G == 8) {
+    const int lo = __builtin_amdgcn_update_dpp(x, x, 0x150 + I, 0xf, 0x3, false);
+    return __builtin_amdgcn_update_dpp(lo, x, 0x158 + I, 0xf, 0xc, false);
+  } else if constexpr (G == 4) {
+    return __builtin_amdgcn_update_dpp(x, x, I * 0x55, 0xf, 0xf, false);   // quad_perm:[I,I,I,I]
+  } else if constexpr (G == 2) {
+    return __builtin_amdgcn_update_dpp(x, x, I ? 0xF5 : 0xA0, 0xf, 0xf, false);
+  } else {
+    return x;
+  }
+}
+template <int G, int I>
+__device__ inline float tile_get(float x) {
+  return __int_as_float(tile_get<G, I>(__float_as_int(x)));
+}
+template <int G, int I>
+__device__ inline int64_t tile_get(int64_t x) {
+  const uint32_t lo = (uint32_t)tile_get<G, I>((int)x);
+  return ((int64_t)tile_get<G, I>((int)(x >> 32)) << 32) | lo;
+}
+// Sums of a tile's values over the G lanes of an edge: the lane that holds edge i gets v[i]'s.
+template <int G>
+__device__ inline float tile_scatter(float (&v)[kTile<G>], int lane) {
+  constexpr int N = kTile<G>;
+  auto level = [&](auto B, auto ctrl) {   // partners differ in lane bit B (and agree on the halves)
+    constexpr int half = 1 << decltype(B)::value;
+    if constexpr (half < N) {
+      const bool up = lane & half;
+#pragma unroll
+      for (int j = 0; j < half; ++j) {
+        const float send = up ? v[j] : v[half + j], keep = up ? v[half + j] : v[j];
+        v[j] = keep + dpp<decltype(ctrl)::value>(send);
+      }
+    }
+  };
+  level(std::integral_constant<int, 3>(), std::integral_constant<int, 0x140>());
+  level(std::integral_constant<int, 2>(), std::integral_constant<int, 0x141>());
+  level(std::integral_constant<int, 1>(), std::integral_constant<int, 0x4E>());
+  level(std::integral_constant<int, 0>(), std::integral_constant<int, 0xB1>());
+  if constexpr (G == 32) {
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[0]), __float_as_uint(v[0]), false,
+                                              false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+  return v[0];
+}
+// f(integral_constant 0), ..., f(N - 1)
+template <typename F, int... I>
+__device__ inline void each_(F&& f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>()), ...);
+}
+template <int N, typename F>
+__device__ inline void each(F&& f) {
+  each_(f, std::make_integer_sequence<int, N>());
+}
+
 // ------------------------------------------------------------------ work items
-// Which (row, head, edges) a group of `gs` lanes has.
+// Which (row, head, edges) a group of `gs` lanes has. Counts are below 2^31 (checked at launch).
 struct Work {
-  // plain rows: units of `chunk` rows of one head, dealt to the XCDs in turn
-  int64_t rows;
-  int heads, chunk, gs;
-  int64_t units;            // ceil(rows / chunk) * heads
-  int blocks_per_unit;
+  // plain rows: units of 2^chunk_log blocks' rows of one head, dealt to the XCDs in turn
+  int rows, heads, gs, gs_log, unit_log;
+  int units;                       // row chunks * heads
   const int32_t* rowptr;
   // pieces: of hub rows (hubs != NULL: the plan's entries), or of the rows of a serving call
   // (nodes != NULL: `pieces` of each)
   int hub_edges;
   const int32_t *hubs, *hub_count;
-  int64_t hub_bound, hub_blocks;   // blocks [0, hub_blocks) have the pieces
+  int hub_bound, hub_blocks;       // blocks [0, hub_blocks) have the pieces
   const int64_t* nodes;
   int pieces;
   int64_t num_nodes;
 };
 struct Item {
-  int64_t row;    // of the outputs and of q; < 0: none
-  int64_t slot;   // of the partial results; < 0: this item is the whole row
-  int head, beg, end;
+  int row;        // of the outputs and of q; < 0: none
+  int slot;       // of the partial results; < 0: this item is the whole row
+  int head, beg, n;   // its edges: n from beg on
   bool bad;       // a node id that does not exist
 };
 __device__ inline Item find_item(const Work& w) {
-  const int per_block = 256 / w.gs, grp = (int)threadIdx.x / w.gs;
+  const int grp_log = 8 - w.gs_log, grp = (int)threadIdx.x >> w.gs_log;
   Item it = {-1, -1, 0, 0, 0, false};
   if (w.nodes) {
-    const int64_t i = (int64_t)blockIdx.x * per_block + grp;
-    if (i >= w.rows * w.heads * w.pieces) return it;
-    const int64_t rh = i / w.pieces;
+    const uint32_t i = (blockIdx.x << grp_log) + grp, rh = i / (uint32_t)w.pieces;
+    const uint32_t row = rh / (uint32_t)w.heads;
+    if (row >= (uint32_t)w.rows) return it;
+    it.row = (int)row;
+    it.head = (int)(rh - row * w.heads);
     const int piece = (int)(i - rh * w.pieces);
-    it.row = rh / w.heads;
-    it.head = (int)(rh - it.row * w.heads);
     it.slot = w.pieces > 1 ? it.row * w.pieces + piece : -1;
     const int64_t n = w.nodes[it.row];
     it.bad = n < 0 || n >= w.num_nodes;
     if (it.bad) return it;
-    const int b = w.rowptr[n], e = w.rowptr[n + 1];
-    const int len = (int)(((int64_t)e - b + w.pieces - 1) / w.pieces);
-    it.beg = (int)min((int64_t)e, b + (int64_t)piece * len);
-    it.end = (int)min((int64_t)e, (int64_t)it.beg + len);
+    const int b = w.rowptr[n], deg = w.rowptr[n + 1] - b;
+    const int64_t len = ((int64_t)deg + w.pieces - 1) / w.pieces, at = min((int64_t)deg, piece * len);
+    it.beg = b + (int)at;
+    it.n = (int)min(len, deg - at);
     return it;
   }
-  if (blockIdx.x < w.hub_blocks) {
-    const int64_t i = (int64_t)blockIdx.x * per_block + grp;
-    const int64_t pc = i / w.heads;
-    if (pc >= w.hub_bound || pc >= *w.hub_count) return it;
-    const int32_t* hp = w.hubs + 4 * pc;
+  if ((int)blockIdx.x < w.hub_blocks) {
+    const uint32_t i = (blockIdx.x << grp_log) + grp, pc = i / (uint32_t)w.heads;
+    if (pc >= (uint32_t)w.hub_bound || (int)pc >= *w.hub_count) return it;
+    const int32_t* hp = w.hubs + 4 * (int64_t)pc;
     it.row = hp[0];
     it.head = (int)(i - pc * w.heads);
-    it.slot = pc;
-    it.beg = w.rowptr[it.row] + hp[1] * w.hub_edges;
-    it.end = (int)min((int64_t)w.rowptr[it.row + 1], (int64_t)it.beg + w.hub_edges);
+    it.slot = (int)pc;
+    const int b = w.rowptr[it.row], deg = w.rowptr[it.row + 1] - b, at = hp[1] * w.hub_edges;
+    it.beg = b + at;
+    it.n = min(w.hub_edges, deg - at);
     return it;
   }
-  const int64_t b = blockIdx.x - w.hub_blocks;
-  const int64_t j = b / 8;
-  const int64_t unit = j / w.blocks_per_unit * 8 + b % 8;
-  if (unit >= w.units) return it;
-  const int64_t ck = unit / w.heads;
-  const int64_t in = (j % w.blocks_per_unit) * per_block + grp;
-  const int64_t row = ck * w.chunk + in;
-  if (in >= w.chunk || row >= w.rows) return it;
+  const uint32_t b = blockIdx.x - w.hub_blocks, j = b >> 3;
+  const uint32_t unit = (j >> w.unit_log << 3) + (b & 7);
+  if (unit >= (uint32_t)w.units) return it;
+  const uint32_t ck = unit / (uint32_t)w.heads;
+  const uint32_t block = (ck << w.unit_log) + (j & ((1u << w.unit_log) - 1));
+  const uint32_t row = (block << grp_log) + grp;
+  if (row >= (uint32_t)w.rows) return it;
   it.head = (int)(unit - ck * w.heads);
   it.beg = w.rowptr[row];
-  it.end = w.rowptr[row + 1];
-  if (w.hub_edges > 0 && it.end - it.beg > w.hub_edges) return it;   // in pieces, above
-  it.row = row;
+  const int n = w.rowptr[row + 1] - it.beg;
+  if (w.hub_edges > 0 && n > w.hub_edges) return it;   // in pieces, above
+  it.n = n;
+  it.row = (int)row;
   return it;
 }
 
@@ -279,7 +359,7 @@ struct AttnArgs {
   float2* S;                 // [H][E] logits
   float4* stat;              // [H][rows] {max1, 1/sum1, max2, 1/sum2}
   void* out;
-  float* part;               // [slot][H][part_width]
+  float* part;               // [slot][H][...], [part_width] of the sums
   int part_width;
   // backward
   float* dw;                 // [H][E]
@@ -288,6 +368,43 @@ struct AttnArgs {
   void *gq, *gk, *gv;
 };
 
+// A lane's place in its row's group, and its chunks' columns. Lanes past a row's last chunk read that
+// one again (no branch around a load); their part of a dot product is dropped (in_d, in_dv), and
+// what they add up is not stored.
+template <int G, int NV>
+struct Lane {
+  int c, slot, slots, at_d, at_dv[NV];
+  bool in_d, in_dv[NV];
+  __device__ Lane(int gs, int dp, int dvp) {
+    const int lane = threadIdx.x & (gs - 1);
+    c = lane & (G - 1);
+    slot = lane / G;
+    slots = gs / G;
+    in_d = c * 8 < dp;
+    at_d = min(c * 8, dp - 8);
+    for (int i = 0; i < NV; ++i) {
+      in_dv[i] = (c + i * G) * 8 < dvp;
+      at_dv[i] = min((c + i * G) * 8, dvp - 8);
+    }
+  }
+};
+// Turns of `step` edges that cover the longest of the wave's rows.
+__device__ inline int turns_of(int n, int step) { return (n + step - 1) / step; }
+// Edge number o of an item. Past its end: its first edge again (index 0 of every array where it has
+// none at all), to be left out by `in`.
+struct Edge {
+  bool in;
+  int e;       // CSR slot
+  int64_t j;   // the other node
+  __device__ Edge(const Item& it, int o, const int32_t* col) {
+    in = o < it.n;
+    e = it.n > 0 ? it.beg + (in ? o : 0) : 0;
+    const int c = col[e];
+    j = it.n > 0 ? c : 0;
+  }
+};
+constexpr int kFlight = 4;   // edges whose rows are in flight per slot
+
 // One row's state over a slot's edges: both maps' running maximum and sum.
 template <int NV>
 struct Acc {
@@ -295,19 +412,26 @@ struct Acc {
   float a1[NV][8] = {}, a2[NV][8] = {};
 };
 __device__ inline float finite_max(float m) { return m == -kInf ? 0.f : m; }
+// {max, 1 / sum} of both maps; nothing open: weights of 0
+__device__ inline float4 row_stat(float m1, float s1, float m2, float s2) {
+  return make_float4(finite_max(m1), s1 == 0.f ? 0.f : 1.f / s1, finite_max(m2),
+                     s2 == 0.f ? 0.f : 1.f / s2);
+}
 
 // U edges of a slot. CHECK: some lane of the wave has an edge that is past its row's end or shut;
 // what such an edge points at is not let into the sums.
 template <typename T, int G, int NV, int U, bool BIAS, bool CHECK>
-__device__ inline void forward_step(const Raw<T> (&k1)[U], const Raw<T> (&k2)[U],
+__device__ inline void serve_step(const Raw<T> (&k1)[U], const Raw<T> (&k2)[U],
                                     const Raw<T> (&v)[U][NV], const Raw<T>& q1, const Raw<T>& q2,
-                                    const float (&b)[U], const bool (&open)[U], float scale,
-                                    Acc<NV>& acc, float2 (&x)[U]) {
+                                    const float (&b)[U], const bool (&open)[U], bool in_d,
+                                    float scale, Acc<NV>& acc) {
+  float2 x[U];
   float n1 = acc.m1, n2 = acc.m2;
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    x[u].x = edge_sum<G>(dot8(q1, k1[u], 0.f)) * scale;
-    x[u].y = edge_sum<G>(dot8(q2, k2[u], 0.f)) * scale;
+    const float s1 = dot8(q1, k1[u], 0.f), s2 = dot8(q2, k2[u], 0.f);
+    x[u].x = edge_sum<G>(in_d ? s1 : 0.f) * scale;
+    x[u].y = edge_sum<G>(in_d ? s2 : 0.f) * scale;
     if (BIAS) {
       x[u].x += b[u];
       x[u].y += b[u];
@@ -347,87 +471,65 @@ __device__ inline void forward_step(const Raw<T> (&k1)[U], const Raw<T> (&k2)[U]
   }
 }
 
-// Edges in flight per slot
-template <typename T>
-struct Unroll {
-  static constexpr int kForward = sizeof(T) == 4 ? 2 : 4;
-};
-
-template <typename T, int G, int NV, bool BIAS, bool SAVE>
-__global__ void __launch_bounds__(256) diff_forward_kernel(AttnArgs a) {
-  constexpr int U = Unroll<T>::kForward;
+// The serving form: one pass with running maxima and sums, each slot its own edges.
+template <typename T, int G, int NV, bool BIAS>
+__global__ void __launch_bounds__(256) diff_serve_kernel(AttnArgs a) {
+  constexpr int U = sizeof(T) == 4 ? 2 : 4;
   const Item it = find_item(a.w);
-  const int gs = a.w.gs, lane = threadIdx.x & (gs - 1);
-  const int c = lane % G, slot = lane / G, slots = gs / G;
-  const int dch = a.dp / 8, vch = a.dvp / 8;
+  const Lane<G, NV> l(a.w.gs, a.dp, a.dvp);
   const bool has = it.row >= 0;
   const int64_t row = has ? it.row : 0;
-  Raw<T> q1 = zero8<T>(), q2 = zero8<T>();
-  if (has && c < dch) {
-    const T* q = (const T*)a.q + row * a.ldq + (int64_t)it.head * 2 * a.dp + c * 8;
-    q1 = load8(q);
-    q2 = load8(q + a.dp);
-  }
+  const T* qr = (const T*)a.q + row * a.ldq + (int64_t)it.head * 2 * a.dp + l.at_d;
+  const Raw<T> q1 = load8(qr), q2 = load8(qr + a.dp);
   Acc<NV> acc;
-  const T* kb = (const T*)a.k + (int64_t)it.head * 2 * a.dp + c * 8;
-  const T* vb = (const T*)a.v + (int64_t)it.head * a.dvp + c * 8;
-  const int n = has ? it.end - it.beg : 0;
-  const int turns = wave_max((n + slots * U - 1) / (slots * U));
+  const T* kb = (const T*)a.k + (int64_t)it.head * 2 * a.dp + l.at_d;
+  const T* vb = (const T*)a.v + (int64_t)it.head * a.dvp;
+  const int turns = turns_of(wave_max(it.n), l.slots * U);
   for (int t = 0; t < turns; ++t) {
     Raw<T> k1[U], k2[U], v[U][NV];
     float b[U];
     bool open[U], all = true;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int o = (t * U + u) * slots + slot;
-      open[u] = o < n;
-      // past the end: the row's first edge (row 0 where there is none), kept out by CHECK
-      const int e = open[u] ? it.beg + o : it.beg;
-      const int64_t j = n > 0 ? a.col[e] : 0;
+      const Edge e(it, (t * U + u) * l.slots + l.slot, a.col);
+      open[u] = e.in;
       b[u] = 0.f;
-      if (BIAS && n > 0) {
-        b[u] = a.bias[(int)a.bucket[e] * a.w.heads + it.head];
+      if (BIAS) {
+        const int bk = a.bucket[e.e];   // (past the end: not necessarily one)
+        b[u] = a.bias[(e.in ? bk : 0) * a.w.heads + it.head];
         open[u] = open[u] && b[u] != -kInf;
       }
       all = all && open[u];
-      k1[u] = k2[u] = zero8<T>();
-      if (c < dch) {
-        k1[u] = load8(kb + j * a.ldk);
-        k2[u] = load8(kb + j * a.ldk + a.dp);
-      }
+      k1[u] = load8(kb + e.j * a.ldk);
+      k2[u] = load8(kb + e.j * a.ldk + a.dp);
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        v[u][i] = zero8<T>();
-        if (c + i * G < vch) v[u][i] = load8(vb + j * a.ldv + i * G * 8);
-      }
+      for (int i = 0; i < NV; ++i) v[u][i] = load8(vb + e.j * a.ldv + l.at_dv[i]);
     }
-    float2 x[U];
     if (__all(all))
-      forward_step<T, G, NV, U, BIAS, false>(k1, k2, v, q1, q2, b, open, a.scale, acc, x);
+      serve_step<T, G, NV, U, BIAS, false>(k1, k2, v, q1, q2, b, open, l.in_d, a.scale, acc);
     else
-      forward_step<T, G, NV, U, BIAS, true>(k1, k2, v, q1, q2, b, open, a.scale, acc, x);
-    if (SAVE && c == 0) {
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int o = (t * U + u) * slots + slot;
-        if (o < n) a.S[(int64_t)it.head * a.E + it.beg + o] = x[u];
-      }
-    }
+      serve_step<T, G, NV, U, BIAS, true>(k1, k2, v, q1, q2, b, open, l.in_d, a.scale, acc);
   }
   // the slots joined
-  const float m1 = slots_max<G>(acc.m1, gs), m2 = slots_max<G>(acc.m2, gs);
+  const int c = l.c, slot = l.slot;
+  const float m1 = slots_max<G>(acc.m1, a.w.gs), m2 = slots_max<G>(acc.m2, a.w.gs);
   const float c1 = exp_(acc.m1 - finite_max(m1)), c2 = exp_(acc.m2 - finite_max(m2));
-  const float l1 = slots_sum<G>(acc.l1 * c1, gs), l2 = slots_sum<G>(acc.l2 * c2, gs);
+  float ls[2] = {acc.l1 * c1, acc.l2 * c2};
+  slots_sum<G>(ls, a.w.gs);
+  const float l1 = ls[0], l2 = ls[1];
 #pragma unroll
-  for (int j = 0; j < NV; ++j)
+  for (int j = 0; j < NV; ++j) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      acc.a1[j][i] = slots_sum<G>(acc.a1[j][i] * c1, gs);
-      acc.a2[j][i] = slots_sum<G>(acc.a2[j][i] * c2, gs);
+      acc.a1[j][i] *= c1;
+      acc.a2[j][i] *= c2;
     }
+    slots_sum<G>(acc.a1[j], a.w.gs);
+    slots_sum<G>(acc.a2[j], a.w.gs);
+  }
   if (!has || slot != 0) return;
   if (it.slot >= 0) {   // a piece: {m1, l1, m2, l2, sums of map 1, of map 2}
-    float* p = a.part + (it.slot * a.w.heads + it.head) * a.part_width;
+    float* p = a.part + ((int64_t)it.slot * a.w.heads + it.head) * a.part_width;
     if (c == 0) *(float4*)p = make_float4(m1, it.bad ? __builtin_nanf("") : l1, m2, l2);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
@@ -438,9 +540,6 @@ __global__ void __launch_bounds__(256) diff_forward_kernel(AttnArgs a) {
   }
   const float i1 = l1 == 0.f ? 0.f : 1.f / l1, i2 = l2 == 0.f ? 0.f : 1.f / l2;
   const float w2 = a.lam[it.head] * i2;
-  if (SAVE && c == 0)
-    a.stat[(int64_t)it.head * a.w.rows + row] =
-        make_float4(finite_max(m1), i1, finite_max(m2), i2);
   T* out = (T*)a.out + (row * a.w.heads + it.head) * a.dv;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
@@ -454,27 +553,13 @@ __global__ void __launch_bounds__(256) diff_forward_kernel(AttnArgs a) {
   }
 }
 
-// The pieces of a row joined in order: a workgroup per (row, head), 4 runs of pieces side by side.
+// The pieces of a served row joined in order: a workgroup per (row, head), 4 runs of pieces side by
+// side.
 template <typename T>
-__global__ void __launch_bounds__(1024) diff_join_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(1024) diff_serve_join_kernel(AttnArgs a) {
   extern __shared__ __attribute__((aligned(16))) float lds[];   // [4][2 dvp]
-  int64_t row, first;
-  int head, pieces;
-  if (a.w.nodes) {
-    row = blockIdx.x / a.w.heads;
-    head = (int)(blockIdx.x - row * a.w.heads);
-    first = row * a.w.pieces;
-    pieces = a.w.pieces;
-  } else {
-    const int64_t pc = blockIdx.x / a.w.heads;
-    if (pc >= *a.w.hub_count) return;
-    const int32_t* hp = a.w.hubs + 4 * pc;
-    if (hp[1] != 0) return;   // a hub's first entry speaks for it
-    row = hp[0];
-    head = (int)(blockIdx.x - pc * a.w.heads);
-    pieces = hp[2];
-    first = pc;
-  }
+  const int64_t row = blockIdx.x / a.w.heads, first = row * a.w.pieces;
+  const int head = (int)(blockIdx.x - row * a.w.heads), pieces = a.w.pieces;
   const int H = a.w.heads;
   const float* p0 = a.part + (first * H + head) * a.part_width;
   const int64_t step = (int64_t)H * a.part_width;
@@ -517,11 +602,9 @@ __global__ void __launch_bounds__(1024) diff_join_kernel(AttnArgs a) {
     }
     out[x] = (T)(s1 * i1 - s2 * w2);
   }
-  if (a.stat && threadIdx.x == 0)
-    a.stat[(int64_t)head * a.w.rows + row] = make_float4(r1, i1, r2, i2);
 }
 
-// ------------------------------------------------------------------ backward
+// ------------------------------------------------------------------ forward over whole rows
 // Both maps' weights of an edge from its logits; a shut or -inf logit has weight 0 whatever the
 // statistics hold.
 __device__ inline float2 weights(float2 x, const float4& st) {
@@ -529,204 +612,411 @@ __device__ inline float2 weights(float2 x, const float4& st) {
                      x.y == -kInf ? 0.f : exp_(x.y - st.z) * st.w);
 }
 
+// An item's pass over its edges in tiles: `first` of a tile's first edge in this slot, turn by turn.
+template <int G>
+struct Tiles {
+  int lane, mine, step, most;   // mine: the edge of a tile this lane holds
+  bool owner;                   // (of G = 32 lanes the second 16 hold the first's edges again)
+  __device__ Tiles(const Item& it, int gs) {
+    lane = threadIdx.x & 63;
+    mine = lane & (kTile<G> - 1);
+    owner = G < 32 || (lane & 31) < 16;
+    step = gs / G * kTile<G>;
+    most = wave_max(it.n);
+  }
+  __device__ int first(int t, int slot) const { return t * step + slot * kTile<G>; }
+  // no lane of the wave has an edge from number i of its tile on
+  __device__ bool done(int t, int i) const { return t * step + i >= most; }
+};
+
+// The logits of every edge and the softmax statistics of every row.
+template <typename T, int G, bool BIAS>
+__global__ void __launch_bounds__(256) diff_score_kernel(AttnArgs a) {
+  constexpr int NL = kTile<G>, U = NL < kFlight ? NL : kFlight;
+  const Item it = find_item(a.w);
+  const Lane<G, 1> l(a.w.gs, a.dp, 8);
+  const Tiles<G> tl(it, a.w.gs);
+  const bool has = it.row >= 0;
+  const int64_t row = has ? it.row : 0;
+  const T* qr = (const T*)a.q + row * a.ldq + (int64_t)it.head * 2 * a.dp + l.at_d;
+  const Raw<T> q1 = load8(qr), q2 = load8(qr + a.dp);
+  const T* kb = (const T*)a.k + (int64_t)it.head * 2 * a.dp + l.at_d;
+  const int64_t he = (int64_t)it.head * a.E;
+  float m1 = -kInf, m2 = -kInf, s1 = 0.f, s2 = 0.f;
+  for (int t = 0; !tl.done(t, 0); ++t) {
+    const int o = tl.first(t, l.slot) + tl.mine;
+    const Edge e(it, o, a.col);
+    const int64_t off = e.j * a.ldk;
+    float b = 0.f;
+    if (BIAS) {
+      const int bk = a.bucket[e.e];   // (past the end: not necessarily one)
+      b = a.bias[(e.in ? bk : 0) * a.w.heads + it.head];
+    }
+    float x1[NL], x2[NL];
+    each<NL / U>([&](auto B) {
+      constexpr int b0 = decltype(B)::value * U;
+      if (b0 > 0 && tl.done(t, b0)) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) x1[b0 + u] = x2[b0 + u] = 0.f;
+        return;
+      }
+      Raw<T> k1[U], k2[U];
+      each<U>([&](auto I) {
+        constexpr int u = decltype(I)::value;
+        const T* p = kb + tile_get<G, b0 + u>(off);
+        k1[u] = load8(p);
+        k2[u] = load8(p + a.dp);
+      });
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float d1 = dot8(q1, k1[u], 0.f), d2 = dot8(q2, k2[u], 0.f);
+        x1[b0 + u] = l.in_d ? d1 : 0.f;
+        x2[b0 + u] = l.in_d ? d2 : 0.f;
+      }
+    });
+    float2 x;
+    x.x = fmaf(tile_scatter<G>(x1, tl.lane), a.scale, b);
+    x.y = fmaf(tile_scatter<G>(x2, tl.lane), a.scale, b);
+    const bool shut = !e.in || (BIAS && b == -kInf);
+    x.x = shut ? -kInf : x.x;
+    x.y = shut ? -kInf : x.y;
+    if (tl.owner) {
+      if (e.in) a.S[he + e.e] = x;
+      const float n1 = fmaxf(m1, x.x), n2 = fmaxf(m2, x.y);
+      const float r1 = finite_max(n1), r2 = finite_max(n2);
+      s1 = s1 * exp_(m1 - r1) + exp_(x.x - r1);
+      s2 = s2 * exp_(m2 - r2) + exp_(x.y - r2);
+      m1 = n1;
+      m2 = n2;
+    }
+  }
+  // the lanes joined
+  const float t1 = slots_max<1>(m1, a.w.gs), t2 = slots_max<1>(m2, a.w.gs);
+  float s[2] = {s1 * exp_(m1 - finite_max(t1)), s2 * exp_(m2 - finite_max(t2))};
+  slots_sum<1>(s, a.w.gs);
+  if (!has || l.c != 0 || l.slot != 0) return;
+  if (it.slot >= 0)
+    *(float4*)(a.part + ((int64_t)it.slot * a.w.heads + it.head) * 4) =
+        make_float4(t1, s[0], t2, s[1]);
+  else
+    a.stat[(int64_t)it.head * a.w.rows + row] = row_stat(t1, s[0], t2, s[1]);
+}
+
+// out of every row: its values weighted by p_1 - lam p_2.
+template <typename T, int G, int NV>
+__global__ void __launch_bounds__(256) diff_value_kernel(AttnArgs a) {
+  constexpr int NL = kTile<G>, U = NL < kFlight ? NL : kFlight;
+  const Item it = find_item(a.w);
+  const Lane<G, NV> l(a.w.gs, a.dp, a.dvp);
+  const Tiles<G> tl(it, a.w.gs);
+  const bool has = it.row >= 0;
+  const int64_t row = has ? it.row : 0;
+  const float4 st = a.stat[(int64_t)it.head * a.w.rows + row];
+  const float lam = a.lam[it.head];
+  const T* vb = (const T*)a.v + (int64_t)it.head * a.dvp;
+  const int64_t he = (int64_t)it.head * a.E;
+  float acc[NV][8] = {};
+  for (int t = 0; !tl.done(t, 0); ++t) {
+    const Edge e(it, tl.first(t, l.slot) + tl.mine, a.col);
+    const int64_t off = e.j * a.ldv;
+    const float2 x = a.S[he + e.e], p = weights(x, st);
+    const int open = e.in && (x.x != -kInf || x.y != -kInf);
+    const float w = open ? p.x - lam * p.y : 0.f;
+    auto edges = [&](auto ALL) {
+      each<NL / U>([&](auto B) {
+        constexpr int b0 = decltype(B)::value * U;
+        if (b0 > 0 && tl.done(t, b0)) return;
+        Raw<T> v[U][NV];
+        each<U>([&](auto I) {
+          constexpr int u = decltype(I)::value;
+          const T* p = vb + tile_get<G, b0 + u>(off);
+#pragma unroll
+          for (int i = 0; i < NV; ++i) v[u][i] = load8(p + l.at_dv[i]);
+        });
+        each<U>([&](auto I) {
+          constexpr int u = decltype(I)::value;
+          const float wu = tile_get<G, b0 + u>(w);
+          const bool keep = decltype(ALL)::value || tile_get<G, b0 + u>(open);
+#pragma unroll
+          for (int i = 0; i < NV; ++i)
+            axpy8(wu, decltype(ALL)::value ? v[u][i] : keep8(keep, v[u][i]), acc[i]);
+        });
+      });
+    };
+    if (__all(open)) edges(std::true_type());
+    else edges(std::false_type());
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) slots_sum<G>(acc[i], a.w.gs);
+  if (!has || l.slot != 0) return;
+  if (it.slot >= 0) {
+    float* p = a.part + ((int64_t)it.slot * a.w.heads + it.head) * a.part_width;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) store8(p, (l.c + i * G) * 8, a.dvp, true, acc[i]);
+    return;
+  }
+  T* out = (T*)a.out + (row * a.w.heads + it.head) * a.dv;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) store8(out, (l.c + i * G) * 8, a.dv, a.dv == a.dvp, acc[i]);
+}
+
+// The hubs of the plan, in a fixed grid of workgroups: f(first slot, node, pieces, head).
+template <typename F>
+__device__ inline void each_hub(const Work& w, int64_t at, int64_t step, F&& f) {
+  const int64_t n = (int64_t)min(*w.hub_count, w.hub_bound) * w.heads;
+  for (int64_t i = at; i < n; i += step) {
+    const int pc = (int)(i / w.heads);
+    const int32_t* hp = w.hubs + 4 * (int64_t)pc;
+    if (hp[1] == 0) f(pc, hp[0], hp[2], (int)(i - (int64_t)pc * w.heads));   // its first entry
+  }
+}
+// Statistics of the hubs from their pieces'.
+__global__ void __launch_bounds__(256) diff_score_join_kernel(AttnArgs a) {
+  each_hub(a.w, (int64_t)blockIdx.x * 256 + threadIdx.x, (int64_t)gridDim.x * 256,
+           [&](int first, int row, int pieces, int head) {
+             auto part = [&](int k) {
+               return *(const float4*)(a.part + ((int64_t)(first + k) * a.w.heads + head) * 4);
+             };
+             float m1 = -kInf, m2 = -kInf, s1 = 0.f, s2 = 0.f;
+             for (int k = 0; k < pieces; ++k) {
+               m1 = fmaxf(m1, part(k).x);
+               m2 = fmaxf(m2, part(k).z);
+             }
+             for (int k = 0; k < pieces; ++k) {
+               s1 += part(k).y * exp_(part(k).x - finite_max(m1));
+               s2 += part(k).w * exp_(part(k).z - finite_max(m2));
+             }
+             a.stat[(int64_t)head * a.w.rows + row] = row_stat(m1, s1, m2, s2);
+           });
+}
+// Sums of the hubs' pieces: [two maps of dp (where maps_in) | dvp] columns, a thread a column.
+template <typename T>
+__global__ void __launch_bounds__(256) diff_sum_join_kernel(AttnArgs a, int maps_in, T* maps,
+                                                            T* values) {
+  const int W = a.part_width, dp2 = maps_in ? 2 * a.dp : 0;
+  each_hub(a.w, blockIdx.x, gridDim.x, [&](int first, int row, int pieces, int head) {
+    const int64_t rh = (int64_t)row * a.w.heads + head, step = (int64_t)a.w.heads * W;
+    for (int x = threadIdx.x; x < W; x += 256) {
+      const float* p = a.part + ((int64_t)first * a.w.heads + head) * W + x;
+      float s = 0.f;
+#pragma unroll 8
+      for (int k = 0; k < pieces; ++k) s += p[k * step];
+      if (x < dp2) {
+        const int m = x >= a.dp, y = x - m * a.dp;
+        if (maps && y < a.d) maps[(rh * 2 + m) * a.d + y] = (T)s;
+      } else if (values && x - dp2 < a.dv) {
+        values[rh * a.dv + x - dp2] = (T)s;
+      }
+    }
+  });
+}
+
+// ------------------------------------------------------------------ backward
 // A: dw = go . v of every edge, D_1 and D_2 of every row.
 template <typename T, int G, int NV>
 __global__ void __launch_bounds__(256) diff_dw_kernel(AttnArgs a) {
-  constexpr int U = 4;
+  constexpr int NL = kTile<G>, U = NL < kFlight ? NL : kFlight;
   const Item it = find_item(a.w);
-  const int gs = a.w.gs, lane = threadIdx.x & (gs - 1);
-  const int c = lane % G, slot = lane / G, slots = gs / G, vch = a.dvp / 8;
+  const Lane<G, NV> l(a.w.gs, a.dp, a.dvp);
+  const Tiles<G> tl(it, a.w.gs);
   const bool has = it.row >= 0;
   const int64_t row = has ? it.row : 0;
+  const T* gr = (const T*)a.go + row * a.ldgo + (int64_t)it.head * a.dvp;
   Raw<T> g[NV];
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    g[i] = zero8<T>();
-    if (has && c + i * G < vch)
-      g[i] = load8((const T*)a.go + row * a.ldgo + (int64_t)it.head * a.dvp + (c + i * G) * 8);
-  }
+  for (int i = 0; i < NV; ++i) g[i] = load8(gr + l.at_dv[i]);
   const float4 st = a.stat[(int64_t)it.head * a.w.rows + row];
-  const T* vb = (const T*)a.v + (int64_t)it.head * a.dvp + c * 8;
-  const int64_t at = (int64_t)it.head * a.E + it.beg;
-  const int n = has ? it.end - it.beg : 0;
-  const int turns = wave_max((n + slots * U - 1) / (slots * U));
-  float d1 = 0.f, d2 = 0.f;
-  for (int t = 0; t < turns; ++t) {
-    Raw<T> v[U][NV];
-    float2 x[U];
+  const T* vb = (const T*)a.v + (int64_t)it.head * a.dvp;
+  const int64_t he = (int64_t)it.head * a.E;
+  float d[2] = {0.f, 0.f};
+  for (int t = 0; !tl.done(t, 0); ++t) {
+    const Edge e(it, tl.first(t, l.slot) + tl.mine, a.col);
+    const int64_t off = e.j * a.ldv;
+    const float2 x = a.S[he + e.e];
+    float y[NL];
+    each<NL / U>([&](auto B) {
+      constexpr int b0 = decltype(B)::value * U;
+      if (b0 > 0 && tl.done(t, b0)) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int o = (t * U + u) * slots + slot;
-      const int e = o < n ? o : 0;
-      const int64_t j = n > 0 ? a.col[it.beg + e] : 0;
-      x[u] = n > 0 ? a.S[at + e] : make_float2(-kInf, -kInf);
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        v[u][i] = zero8<T>();
-        if (c + i * G < vch) v[u][i] = load8(vb + j * a.ldv + i * G * 8);
+        for (int u = 0; u < U; ++u) y[b0 + u] = 0.f;
+        return;
       }
-    }
+      Raw<T> v[U][NV];
+      each<U>([&](auto I) {
+        constexpr int u = decltype(I)::value;
+        const T* p = vb + tile_get<G, b0 + u>(off);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int o = (t * U + u) * slots + slot;
-      float s = 0.f;
+        for (int i = 0; i < NV; ++i) v[u][i] = load8(p + l.at_dv[i]);
+      });
 #pragma unroll
-      for (int i = 0; i < NV; ++i) s = dot8(g[i], v[u][i], s);
-      s = edge_sum<G>(s);
-      if (x[u].x == -kInf && x[u].y == -kInf) s = 0.f;   // shut: its value does not count
-      const float2 p = weights(x[u], st);
-      if (o < n) {
-        d1 = fmaf(p.x, s, d1);
-        d2 = fmaf(p.y, s, d2);
-        if (c == 0) a.dw[at + o] = s;
+      for (int u = 0; u < U; ++u) {
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          const float p = dot8(g[i], v[u][i], 0.f);
+          s += l.in_dv[i] ? p : 0.f;
+        }
+        y[b0 + u] = s;
       }
+    });
+    float dw = tile_scatter<G>(y, tl.lane);
+    if (x.x == -kInf && x.y == -kInf) dw = 0.f;   // shut: its value does not count
+    if (e.in && tl.owner) {
+      const float2 p = weights(x, st);
+      d[0] = fmaf(p.x, dw, d[0]);
+      d[1] = fmaf(p.y, dw, d[1]);
+      a.dw[he + e.e] = dw;
     }
   }
-  d1 = slots_sum<G>(d1, gs);
-  d2 = slots_sum<G>(d2, gs);
-  if (!has || lane != 0) return;
+  slots_sum<1>(d, a.w.gs);
+  if (!has || l.c != 0 || l.slot != 0) return;
   if (it.slot >= 0)
-    *(float2*)(a.part + (it.slot * a.w.heads + it.head) * 2) = make_float2(d1, d2);
+    *(float2*)(a.part + ((int64_t)it.slot * a.w.heads + it.head) * 2) = make_float2(d[0], d[1]);
   else
-    a.D[(int64_t)it.head * a.w.rows + row] = make_float2(d1, d2);
+    a.D[(int64_t)it.head * a.w.rows + row] = make_float2(d[0], d[1]);
 }
 __global__ void __launch_bounds__(256) diff_dw_join_kernel(AttnArgs a) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t pc = i / a.w.heads;
-  const int head = (int)(i - pc * a.w.heads);
-  if (pc >= a.w.hub_bound || pc >= *a.w.hub_count) return;
-  const int32_t* hp = a.w.hubs + 4 * pc;
-  if (hp[1] != 0) return;
-  float2 d = make_float2(0.f, 0.f);
-  for (int k = 0; k < hp[2]; ++k) {
-    const float2 p = *(const float2*)(a.part + ((pc + k) * a.w.heads + head) * 2);
-    d.x += p.x;
-    d.y += p.y;
-  }
-  a.D[(int64_t)head * a.w.rows + hp[0]] = d;
+  each_hub(a.w, (int64_t)blockIdx.x * 256 + threadIdx.x, (int64_t)gridDim.x * 256,
+           [&](int first, int row, int pieces, int head) {
+             float2 d = make_float2(0.f, 0.f);
+             for (int k = 0; k < pieces; ++k) {
+               const float2 p =
+                   *(const float2*)(a.part + ((int64_t)(first + k) * a.w.heads + head) * 2);
+               d.x += p.x;
+               d.y += p.y;
+             }
+             a.D[(int64_t)head * a.w.rows + row] = d;
+           });
 }
 
 // B: gq of every row, and each edge's record for C and the bias.
 template <typename T, int G>
 __global__ void __launch_bounds__(256) diff_gq_kernel(AttnArgs a) {
-  constexpr int U = 4;
+  constexpr int NL = kTile<G>, U = NL < kFlight ? NL : kFlight;
   const Item it = find_item(a.w);
-  const int gs = a.w.gs, lane = threadIdx.x & (gs - 1);
-  const int c = lane % G, slot = lane / G, slots = gs / G, dch = a.dp / 8;
+  const Lane<G, 1> l(a.w.gs, a.dp, 8);
+  const Tiles<G> tl(it, a.w.gs);
   const bool has = it.row >= 0;
   const int64_t row = has ? it.row : 0, sr = (int64_t)it.head * a.w.rows + row;
   const float4 st = a.stat[sr];
   const float2 D = a.D[sr];
   const float lam = a.lam[it.head];
-  const T* kb = (const T*)a.k + (int64_t)it.head * 2 * a.dp + c * 8;
-  const int64_t at = (int64_t)it.head * a.E + it.beg;
-  const int n = has ? it.end - it.beg : 0;
-  const int turns = wave_max((n + slots * U - 1) / (slots * U));
+  const T* kb = (const T*)a.k + (int64_t)it.head * 2 * a.dp + l.at_d;
+  const int64_t he = (int64_t)it.head * a.E;
   float g1[8] = {}, g2[8] = {};
-  for (int t = 0; t < turns; ++t) {
-    Raw<T> k1[U], k2[U];
-    float2 x[U];
-    float dw[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int o = (t * U + u) * slots + slot;
-      const int e = o < n ? o : 0;
-      const int64_t j = n > 0 ? a.col[it.beg + e] : 0;
-      x[u] = o < n ? a.S[at + e] : make_float2(-kInf, -kInf);
-      dw[u] = n > 0 ? a.dw[at + e] : 0.f;
-      k1[u] = k2[u] = zero8<T>();
-      if (c < dch) {
-        k1[u] = load8(kb + j * a.ldk);
-        k2[u] = load8(kb + j * a.ldk + a.dp);
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int o = (t * U + u) * slots + slot;
-      const bool shut = x[u].x == -kInf && x[u].y == -kInf;   // or past the end
-      const float2 p = weights(x[u], st);
-      const float x1 = shut ? 0.f : p.x * (dw[u] - D.x);
-      const float x2 = shut ? 0.f : -lam * p.y * (dw[u] - D.y);
-      if (c == 0 && o < n)
-        a.rec[at + o] = make_float4(x1 * a.scale, x2 * a.scale, shut ? 0.f : p.x - lam * p.y,
+  for (int t = 0; !tl.done(t, 0); ++t) {
+    const Edge e(it, tl.first(t, l.slot) + tl.mine, a.col);
+    const int64_t off = e.j * a.ldk;
+    const float2 x = a.S[he + e.e], p = weights(x, st);
+    const float dw = a.dw[he + e.e];
+    const int open = e.in && (x.x != -kInf || x.y != -kInf);
+    const float x1 = open ? p.x * (dw - D.x) : 0.f;
+    const float x2 = open ? -lam * p.y * (dw - D.y) : 0.f;
+    if (e.in && tl.owner)
+      a.rec[he + e.e] = make_float4(x1 * a.scale, x2 * a.scale, open ? p.x - lam * p.y : 0.f,
                                     x1 + x2);
-      axpy8(x1, keep8(!shut, k1[u]), g1);
-      axpy8(x2, keep8(!shut, k2[u]), g2);
-    }
+    if (!a.gq) continue;
+    auto edges = [&](auto ALL) {
+      each<NL / U>([&](auto B) {
+        constexpr int b0 = decltype(B)::value * U;
+        if (b0 > 0 && tl.done(t, b0)) return;
+        Raw<T> k1[U], k2[U];
+        each<U>([&](auto I) {
+          constexpr int u = decltype(I)::value;
+          const T* p = kb + tile_get<G, b0 + u>(off);
+          k1[u] = load8(p);
+          k2[u] = load8(p + a.dp);
+        });
+        each<U>([&](auto I) {
+          constexpr int u = decltype(I)::value;
+          const float y1 = tile_get<G, b0 + u>(x1), y2 = tile_get<G, b0 + u>(x2);
+          const bool keep = decltype(ALL)::value || tile_get<G, b0 + u>(open);
+          axpy8(y1, decltype(ALL)::value ? k1[u] : keep8(keep, k1[u]), g1);
+          axpy8(y2, decltype(ALL)::value ? k2[u] : keep8(keep, k2[u]), g2);
+        });
+      });
+    };
+    if (__all(open)) edges(std::true_type());
+    else edges(std::false_type());
   }
+  slots_sum<G>(g1, a.w.gs);
+  slots_sum<G>(g2, a.w.gs);
+  if (!has || l.slot != 0 || !a.gq) return;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    g1[i] = slots_sum<G>(g1[i], gs) * a.scale;
-    g2[i] = slots_sum<G>(g2[i], gs) * a.scale;
+    g1[i] *= a.scale;
+    g2[i] *= a.scale;
   }
-  if (!has || slot != 0 || !a.gq) return;
   if (it.slot >= 0) {
-    float* p = a.part + (it.slot * a.w.heads + it.head) * a.part_width;
-    store8(p, c * 8, a.dp, true, g1);
-    store8(p + a.dp, c * 8, a.dp, true, g2);
+    float* p = a.part + ((int64_t)it.slot * a.w.heads + it.head) * a.part_width;
+    store8(p, l.c * 8, a.dp, true, g1);
+    store8(p + a.dp, l.c * 8, a.dp, true, g2);
   } else {
     T* gq = (T*)a.gq + (row * a.w.heads + it.head) * 2 * a.d;
-    store8(gq, c * 8, a.d, a.d == a.dp, g1);
-    store8(gq + a.d, c * 8, a.d, a.d == a.dp, g2);
+    store8(gq, l.c * 8, a.d, a.d == a.dp, g1);
+    store8(gq + a.d, l.c * 8, a.d, a.d == a.dp, g2);
   }
 }
 
 // C: gk and gv of every source from its out-edges (CSR w.rowptr = srowptr, col = scol).
 template <typename T, int G, int NV>
 __global__ void __launch_bounds__(256) diff_gkv_kernel(AttnArgs a) {
-  constexpr int U = 2;
+  constexpr int NL = kTile<G>, U = NL < 2 ? NL : 2;
   const Item it = find_item(a.w);
-  const int gs = a.w.gs, lane = threadIdx.x & (gs - 1);
-  const int c = lane % G, slot = lane / G, slots = gs / G;
-  const int dch = a.dp / 8, vch = a.dvp / 8;
+  const Lane<G, NV> l(a.w.gs, a.dp, a.dvp);
+  const Tiles<G> tl(it, a.w.gs);
   const bool has = it.row >= 0;
   const int64_t row = has ? it.row : 0;
-  const T* qb = (const T*)a.q + (int64_t)it.head * 2 * a.dp + c * 8;
-  const T* gb = (const T*)a.go + (int64_t)it.head * a.dvp + c * 8;
+  const T* qb = (const T*)a.q + (int64_t)it.head * 2 * a.dp + l.at_d;
+  const T* gb = (const T*)a.go + (int64_t)it.head * a.dvp;
   const float4* rec = a.rec + (int64_t)it.head * a.E;
-  const int n = has ? it.end - it.beg : 0;
-  const int turns = wave_max((n + slots * U - 1) / (slots * U));
   float g1[8] = {}, g2[8] = {}, gv[NV][8] = {};
-  for (int t = 0; t < turns; ++t) {
-    Raw<T> q1[U], q2[U], go[U][NV];
-    float4 r[U];
+  for (int t = 0; !tl.done(t, 0); ++t) {
+    const Edge e(it, tl.first(t, l.slot) + tl.mine, a.col);
+    const int64_t offq = e.j * a.ldq, offg = e.j * a.ldgo;
+    const int id = a.seid[e.e];
+    const float4 r = rec[it.n > 0 ? id : 0];
+    // a shut edge is all zeros: what it points at does not count
+    const int open = e.in && (r.x != 0.f || r.y != 0.f || r.z != 0.f);
+    const float r1 = open ? r.x : 0.f, r2 = open ? r.y : 0.f, rw = open ? r.z : 0.f;
+    auto edges = [&](auto ALL) {
+      each<NL / U>([&](auto B) {
+        constexpr int b0 = decltype(B)::value * U;
+        if (b0 > 0 && tl.done(t, b0)) return;
+        Raw<T> q1[U], q2[U], go[U][NV];
+        each<U>([&](auto I) {
+          constexpr int u = decltype(I)::value;
+          const T* p = qb + tile_get<G, b0 + u>(offq);
+          q1[u] = load8(p);
+          q2[u] = load8(p + a.dp);
+          const T* g = gb + tile_get<G, b0 + u>(offg);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int o = (t * U + u) * slots + slot;
-      const int e = it.beg + (o < n ? o : 0);
-      const int64_t i = n > 0 ? a.col[e] : 0;
-      r[u] = o < n ? rec[a.seid[e]] : make_float4(0.f, 0.f, 0.f, 0.f);
-      q1[u] = q2[u] = zero8<T>();
-      if (c < dch) {
-        q1[u] = load8(qb + i * a.ldq);
-        q2[u] = load8(qb + i * a.ldq + a.dp);
-      }
+          for (int k = 0; k < NV; ++k) go[u][k] = load8(g + l.at_dv[k]);
+        });
+        each<U>([&](auto I) {
+          constexpr int u = decltype(I)::value;
+          constexpr bool all = decltype(ALL)::value;
+          const bool keep = all || tile_get<G, b0 + u>(open);
+          const float w1 = tile_get<G, b0 + u>(r1), w2 = tile_get<G, b0 + u>(r2),
+                      w = tile_get<G, b0 + u>(rw);
+          axpy8(w1, all ? q1[u] : keep8(keep, q1[u]), g1);
+          axpy8(w2, all ? q2[u] : keep8(keep, q2[u]), g2);
 #pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        go[u][k] = zero8<T>();
-        if (c + k * G < vch) go[u][k] = load8(gb + i * a.ldgo + k * G * 8);
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      // a shut edge (or one past the end) is all zeros: what it points at does not count
-      const bool keep = r[u].x != 0.f || r[u].y != 0.f || r[u].z != 0.f;
-      axpy8(r[u].x, keep8(keep, q1[u]), g1);
-      axpy8(r[u].y, keep8(keep, q2[u]), g2);
-#pragma unroll
-      for (int k = 0; k < NV; ++k) axpy8(r[u].z, keep8(keep, go[u][k]), gv[k]);
-    }
+          for (int k = 0; k < NV; ++k) axpy8(w, all ? go[u][k] : keep8(keep, go[u][k]), gv[k]);
+        });
+      });
+    };
+    if (__all(open)) edges(std::true_type());
+    else edges(std::false_type());
   }
+  slots_sum<G>(g1, a.w.gs);
+  slots_sum<G>(g2, a.w.gs);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    g1[i] = slots_sum<G>(g1[i], gs);
-    g2[i] = slots_sum<G>(g2[i], gs);
-#pragma unroll
-    for (int k = 0; k < NV; ++k) gv[k][i] = slots_sum<G>(gv[k][i], gs);
-  }
-  if (!has || slot != 0) return;
+  for (int k = 0; k < NV; ++k) slots_sum<G>(gv[k], a.w.gs);
+  if (!has || l.slot != 0) return;
+  const int c = l.c;
   if (it.slot >= 0) {
-    float* p = a.part + (it.slot * a.w.heads + it.head) * a.part_width;
+    float* p = a.part + ((int64_t)it.slot * a.w.heads + it.head) * a.part_width;
     store8(p, c * 8, a.dp, true, g1);
     store8(p + a.dp, c * 8, a.dp, true, g2);
 #pragma unroll
@@ -745,53 +1035,33 @@ __global__ void __launch_bounds__(256) diff_gkv_kernel(AttnArgs a) {
     for (int k = 0; k < NV; ++k) store8(out, (c + k * G) * 8, a.dv, a.dv == a.dvp, gv[k]);
   }
 }
-// A hub's gradient pieces summed in order: [two maps of dp | dvp] columns, one thread a column.
-template <typename T>
-__global__ void __launch_bounds__(256) diff_grad_join_kernel(AttnArgs a, T* maps, T* values) {
-  const int64_t pc = blockIdx.x / a.w.heads;
-  const int head = (int)(blockIdx.x - pc * a.w.heads);
-  if (pc >= *a.w.hub_count) return;
-  const int32_t* hp = a.w.hubs + 4 * pc;
-  if (hp[1] != 0) return;
-  const int64_t rh = (int64_t)hp[0] * a.w.heads + head;
-  const int64_t step = (int64_t)a.w.heads * a.part_width;
-  for (int x = threadIdx.x; x < a.part_width; x += 256) {
-    const float* p = a.part + (pc * a.w.heads + head) * a.part_width + x;
-    float s = 0.f;
-#pragma unroll 8
-    for (int k = 0; k < hp[2]; ++k) s += p[k * step];
-    if (x < 2 * a.dp) {
-      const int m = x >= a.dp, y = x - m * a.dp;
-      if (maps && y < a.d) maps[(rh * 2 + m) * a.d + y] = (T)s;
-    } else if (values && x - 2 * a.dp < a.dv) {
-      values[rh * a.dv + x - 2 * a.dp] = (T)s;
-    }
-  }
-}
 
 // glam[h] = -sum of D_2 over the rows: a workgroup per (run of rows, head), then the runs in order.
+// In float64: the rows' D_2 have both signs, and their sum is far smaller than they are together.
 constexpr int kLamRuns = 64;
-__global__ void __launch_bounds__(1024) diff_lam_kernel(const float2* D, int64_t rows, int64_t per,
-                                                        float* part, float* glam) {
-  __shared__ float red[16];
+__global__ void __launch_bounds__(256) diff_lam_kernel(const float2* D, int64_t rows, int64_t per,
+                                                       double* part) {
+  __shared__ double red[256];
   const int h = blockIdx.y;
   const int64_t r0 = blockIdx.x * per, r1 = min(rows, r0 + per);
-  float s = 0.f;
+  double s = 0.0;
 #pragma unroll 4
-  for (int64_t r = r0 + threadIdx.x; r < r1; r += 1024) s += D[h * rows + r].y;
-  s = group_sum<64>(s);
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
-  __syncthreads();
-  if (threadIdx.x) return;
-  s = 0.f;
-  for (int i = 0; i < 16; ++i) s += red[i];
-  if (gridDim.x == 1) glam[h] = -s;
-  else part[h * gridDim.x + blockIdx.x] = s;
+  for (int64_t r = r0 + threadIdx.x; r < r1; r += 256) s += (double)D[h * rows + r].y;
+  red[threadIdx.x] = s;
+  for (int d = 128; d > 0; d >>= 1) {
+    __syncthreads();
+    if ((int)threadIdx.x < d) red[threadIdx.x] += red[threadIdx.x + d];
+  }
+  if (threadIdx.x == 0) part[h * gridDim.x + blockIdx.x] = red[0];
 }
-__global__ void __launch_bounds__(64) diff_lam_join_kernel(const float* part, int runs,
+__global__ void __launch_bounds__(64) diff_lam_join_kernel(const double* part, int runs, int heads,
                                                            float* glam) {
-  const float s = group_sum<64>(threadIdx.x < runs ? part[blockIdx.x * runs + threadIdx.x] : 0.f);
-  if (threadIdx.x == 0) glam[blockIdx.x] = -s;
+  const int h = blockIdx.x * 64 + threadIdx.x;
+  if (h >= heads) return;
+  double s = 0.0;
+#pragma unroll 8
+  for (int i = 0; i < runs; ++i) s += part[h * runs + i];
+  glam[h] = (float)-s;
 }
 
 // gbias: each lane adds its edges' dx_1 + dx_2 into a column of its own of an LDS table [bucket]
@@ -931,41 +1201,45 @@ void with_geom(const Geom& g, F&& f) {
     default: nv(std::integral_constant<int, 32>()); break;
   }
 }
-// Lanes of a row: 16, 32 or 64, at least G; `per_row` = its average number of edges.
-int row_lanes(int G, double per_row, int edges_per_slot) {
-  int gs = 16;
-  while (gs < 64 && (gs < G || (double)(gs / G) * edges_per_slot < per_row)) gs <<= 1;
+// Lanes of a row: as few as hold an edge (16 at least), so what a row costs once is spread over its
+// edges and four rows share a wave; more where the rows alone would leave the chip short of waves.
+int row_lanes(int G, int64_t items) {
+  int gs = G > 16 ? G : 16;
+  while (gs < 64 && items * gs < 64 * kWantWaves) gs <<= 1;
   return gs;
 }
 
+int log2i(int x) {
+  int l = 0;
+  while ((1 << l) < x) ++l;
+  return l;
+}
 // The plain rows' grid (and the pieces' blocks ahead of it).
-unsigned plan_rows(Work& w, int64_t rows, int heads, int gs, const int32_t* rowptr, int hub_edges,
-                   const int32_t* hubs, const int32_t* hub_count, int64_t hub_bound) {
+int64_t plan_rows(Work& w, int64_t rows, int heads, int gs, const int32_t* rowptr, int hub_edges,
+                  const int32_t* hubs, const int32_t* hub_count, int64_t hub_bound) {
   w = Work{};
-  w.rows = w.num_nodes = rows;
+  w.rows = (int)rows;
+  w.num_nodes = rows;
   w.heads = heads;
   w.gs = gs;
+  w.gs_log = log2i(gs);
   w.rowptr = rowptr;
   const int per_block = 256 / gs;
   // units of kChunk rows; fewer where that would leave XCDs without one
-  int64_t chunk = std::min<int64_t>(kChunk, ceil_div(rows * heads, 64));
-  chunk = std::max<int64_t>(round_up(chunk, per_block), per_block);
-  w.chunk = (int)chunk;
-  w.units = ceil_div(rows, chunk) * heads;
-  w.blocks_per_unit = (int)(chunk / per_block);
+  const int64_t chunk = std::min<int64_t>(kChunk, ceil_div(rows * heads, 64));
+  w.unit_log = log2i((int)ceil_div(chunk, per_block));
+  const int64_t units = ceil_div(rows, (int64_t)per_block << w.unit_log) * heads;
+  w.units = (int)std::min<int64_t>(units, INT32_MAX);
   if (hub_edges > 0 && hub_bound > 0) {
     w.hub_edges = hub_edges;
     w.hubs = hubs;
     w.hub_count = hub_count;
-    w.hub_bound = hub_bound;
-    w.hub_blocks = ceil_div(hub_bound * heads, per_block);
+    w.hub_bound = (int)hub_bound;
+    w.hub_blocks = (int)std::min<int64_t>(ceil_div(hub_bound * heads, per_block), INT32_MAX);
   }
-  return (unsigned)(w.hub_blocks + round_up(w.units, 8) * w.blocks_per_unit);
+  return w.hub_blocks + (round_up(units, 8) << w.unit_log);
 }
 
-struct Dims {
-  int dtype, heads, d, dv, dp, dvp;
-};
 int check_dims(const char* what, int dtype, int heads, int d, int dv, int64_t E, int64_t rows) {
   GATX_REQUIRE(dtype_ok(dtype), "%s: unknown dtype %d", what, dtype);
   GATX_REQUIRE(heads >= 1 && heads <= 65535, "%s: %d heads", what, heads);
@@ -977,6 +1251,11 @@ int check_dims(const char* what, int dtype, int heads, int d, int dv, int64_t E,
 }
 bool chunked(int dtype, const void* p, int64_t ld) {
   return aligned16(p) && ld * dtype_size(dtype) % 16 == 0;
+}
+// Workgroups of a join over the hubs, `per` (hub, head) pairs each: the plan's size is only bounded
+// on the host, so a fixed number walks what there is.
+unsigned join_blocks(const Work& w, int per) {
+  return (unsigned)std::min<int64_t>(ceil_div((int64_t)w.hub_bound * w.heads, per), 1024);
 }
 #define GATX_GRID(blocks, what)                                                             \
   GATX_REQUIRE((blocks) < (1ll << 31), "%s: too many work items for one launch", what)
@@ -1066,53 +1345,87 @@ extern "C" int gatx_diff_attention(int dtype, const void* q, int64_t ldq, const 
                "diff_attention: rows of q, k, v must be 16-byte aligned (pack them)");
   GATX_REQUIRE(aligned16(out), "diff_attention: out must be 16-byte aligned");
   GATX_REQUIRE(!bias == !bucket, "diff_attention: bias and bucket go together");
-  GATX_REQUIRE(!S == !stat && !(S && nodes), "diff_attention: S and stat go together, not with nodes");
+  GATX_REQUIRE(nodes ? !S && !stat : S && stat,
+               "diff_attention: S and stat hold whole rows' logits (not with nodes)");
   AttnArgs a = {};
   a.q = q; a.k = k; a.v = v; a.ldq = ldq; a.ldk = ldk; a.ldv = ldv;
   a.d = d; a.dv = dv; a.dp = (int)round_up(d, 8); a.dvp = (int)round_up(dv, 8);
   a.col = col; a.E = E; a.scale = scale; a.lam = lam; a.bias = bias; a.bucket = bucket;
   a.S = (float2*)S; a.stat = (float4*)stat; a.out = out;
-  a.part = (float*)part; a.part_width = 2 * a.dvp + 4;
+  a.part = (float*)part;
   const Geom g = attn_geom(d, dv);
-  const double per_row = (double)E / (double)num_nodes;
-  int64_t blocks, slots = 0;
+  hipStream_t st = (hipStream_t)s;
   if (nodes) {
     GATX_REQUIRE(pieces >= 1 && pieces <= 4096, "diff_attention: 1..4096 pieces");
-    a.w.rows = rows; a.w.num_nodes = num_nodes; a.w.heads = heads; a.w.rowptr = rowptr;
+    const int64_t items = rows * heads * pieces;
+    GATX_GRID(items, "diff_attention");
+    GATX_REQUIRE(pieces == 1 || (part && part_bytes >= gatx_diff_attention_part_bytes(
+                                             rows * pieces, heads, a.dvp)),
+                 "diff_attention: workspace too small");
+    a.part_width = 2 * a.dvp + 4;
+    a.w.rows = (int)rows; a.w.num_nodes = num_nodes; a.w.heads = heads; a.w.rowptr = rowptr;
     a.w.nodes = nodes; a.w.pieces = pieces;
-    a.w.gs = pieces > 1 ? 64 : row_lanes(g.G, per_row, 4);
-    slots = pieces > 1 ? rows * pieces : 0;
-    blocks = ceil_div(rows * heads * pieces, 256 / a.w.gs);
-  } else {
-    GATX_REQUIRE(hub_edges == 0 || (hubs && hub_count), "diff_attention: null hub plan");
-    blocks = plan_rows(a.w, rows, heads, row_lanes(g.G, per_row, 4), rowptr, hub_edges, hubs,
-                       hub_count, hub_bound);
-    slots = a.w.hub_blocks ? hub_bound : 0;
+    a.w.gs = pieces > 1 ? 64 : row_lanes(g.G, items);
+    a.w.gs_log = log2i(a.w.gs);
+    const unsigned blocks = (unsigned)ceil_div(items, 256 / a.w.gs);
+    with_dtype(dtype, [&](auto t) {
+      using T = decltype(t);
+      with_geom(g, [&](auto G, auto NV) {
+        constexpr int kG = decltype(G)::value, kNV = decltype(NV)::value;
+        if (bias) diff_serve_kernel<T, kG, kNV, true><<<blocks, 256, 0, st>>>(a);
+        else diff_serve_kernel<T, kG, kNV, false><<<blocks, 256, 0, st>>>(a);
+      });
+      return 0;
+    });
+    GATX_LAUNCH_CHECK("diff_attention_serve");
+    if (pieces > 1) {
+      with_dtype(dtype, [&](auto t) {
+        diff_serve_join_kernel<decltype(t)>
+            <<<(unsigned)(rows * heads), 1024, sizeof(float) * 8 * a.dvp, st>>>(a);
+        return 0;
+      });
+      GATX_LAUNCH_CHECK("diff_attention_serve_join");
+    }
+    return 0;
   }
+  GATX_REQUIRE(hub_edges == 0 || (hubs && hub_count), "diff_attention: null hub plan");
+  const int64_t blocks = plan_rows(a.w, rows, heads, row_lanes(g.G, rows * heads), rowptr,
+                                   hub_edges, hubs, hub_count, hub_bound);
   GATX_GRID(blocks, "diff_attention");
-  GATX_REQUIRE(slots == 0 || (part && part_bytes >= gatx_diff_attention_part_bytes(slots, heads, a.dvp)),
+  GATX_REQUIRE(a.w.hub_blocks == 0 ||
+                   (part && part_bytes >= gatx_diff_attention_part_bytes(hub_bound, heads, a.dvp)),
                "diff_attention: workspace too small");
-  hipStream_t st = (hipStream_t)s;
   with_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    with_geom(g, [&](auto G, auto NV) {
-      constexpr int kG = decltype(G)::value, kNV = decltype(NV)::value;
-      if (bias && S) diff_forward_kernel<T, kG, kNV, true, true><<<(unsigned)blocks, 256, 0, st>>>(a);
-      else if (bias) diff_forward_kernel<T, kG, kNV, true, false><<<(unsigned)blocks, 256, 0, st>>>(a);
-      else if (S) diff_forward_kernel<T, kG, kNV, false, true><<<(unsigned)blocks, 256, 0, st>>>(a);
-      else diff_forward_kernel<T, kG, kNV, false, false><<<(unsigned)blocks, 256, 0, st>>>(a);
+    with_geom(Geom{g.G, 1}, [&](auto G, auto) {
+      constexpr int kG = decltype(G)::value;
+      if (bias) diff_score_kernel<T, kG, true><<<(unsigned)blocks, 256, 0, st>>>(a);
+      else diff_score_kernel<T, kG, false><<<(unsigned)blocks, 256, 0, st>>>(a);
     });
     return 0;
   });
-  GATX_LAUNCH_CHECK("diff_attention");
-  if (slots > 0) {
-    const int64_t joins = (nodes ? rows : hub_bound) * heads;
-    GATX_GRID(joins, "diff_attention");
+  GATX_LAUNCH_CHECK("diff_attention_score");
+  if (a.w.hub_blocks) {
+    diff_score_join_kernel<<<join_blocks(a.w, 256), 256, 0, st>>>(a);
+    GATX_LAUNCH_CHECK("diff_attention_score_join");
+  }
+  a.part_width = a.dvp;
+  with_dtype(dtype, [&](auto t) {
+    using T = decltype(t);
+    with_geom(g, [&](auto G, auto NV) {
+      diff_value_kernel<T, decltype(G)::value, decltype(NV)::value>
+          <<<(unsigned)blocks, 256, 0, st>>>(a);
+    });
+    return 0;
+  });
+  GATX_LAUNCH_CHECK("diff_attention_value");
+  if (a.w.hub_blocks) {
     with_dtype(dtype, [&](auto t) {
-      diff_join_kernel<decltype(t)><<<(unsigned)joins, 1024, sizeof(float) * 8 * a.dvp, st>>>(a);
+      using T = decltype(t);
+      diff_sum_join_kernel<T><<<join_blocks(a.w, 1), 256, 0, st>>>(a, 0, nullptr, (T*)out);
       return 0;
     });
-    GATX_LAUNCH_CHECK("diff_attention_join");
+    GATX_LAUNCH_CHECK("diff_attention_value_join");
   }
   return 0;
 }
@@ -1136,7 +1449,7 @@ BackwardLayout backward_layout(int64_t N, int64_t E, int H, int dp, int dvp, int
   l.rec = take(he * sizeof(float4));
   l.dw = take(he * sizeof(float));
   l.D = take(hn * sizeof(float2));
-  l.lam = take(sizeof(float) * kLamRuns * H);
+  l.lam = take(sizeof(double) * kLamRuns * H);
   l.bias = take(nb ? sizeof(float) * bias_runs(E) * H * nb : 0);
   l.part = take(sizeof(float) * std::max((size_t)hub_bound * H * (2 * dp),
                                          (size_t)src_hub_bound * H * (2 * dp + dvp)));
@@ -1200,8 +1513,7 @@ extern "C" int gatx_diff_attention_backward(
   a.part = (float*)(ws + l.part);
   a.gq = gq; a.gk = gk; a.gv = gv;
   const Geom g = attn_geom(d, dv);
-  const double per_row = (double)E / (double)N;
-  const int gs = row_lanes(g.G, per_row, 4);
+  const int gs = row_lanes(g.G, N * heads);
   // A
   int64_t blocks = plan_rows(a.w, N, heads, gs, rowptr, hub_edges, hubs, hub_count, hub_bound);
   GATX_GRID(blocks, "diff_attention_backward");
@@ -1215,15 +1527,15 @@ extern "C" int gatx_diff_attention_backward(
   });
   GATX_LAUNCH_CHECK("diff_attention_dw");
   if (a.w.hub_blocks) {
-    diff_dw_join_kernel<<<(unsigned)ceil_div(hub_bound * heads, 256), 256, 0, st>>>(a);
+    diff_dw_join_kernel<<<join_blocks(a.w, 256), 256, 0, st>>>(a);
     GATX_LAUNCH_CHECK("diff_attention_dw_join");
   }
   if (glam) {
-    const int runs = (int)std::min<int64_t>(kLamRuns, ceil_div(N, 8192));
-    float* lp = (float*)(ws + l.lam);
-    diff_lam_kernel<<<dim3(runs, heads), 1024, 0, st>>>(a.D, N, ceil_div(N, runs), lp, glam);
+    const int runs = (int)std::min<int64_t>(kLamRuns, ceil_div(N, 1024));
+    double* lp = (double*)(ws + l.lam);
+    diff_lam_kernel<<<dim3(runs, heads), 256, 0, st>>>(a.D, N, ceil_div(N, runs), lp);
     GATX_LAUNCH_CHECK("diff_attention_lam");
-    if (runs > 1) diff_lam_join_kernel<<<heads, 64, 0, st>>>(lp, runs, glam);
+    diff_lam_join_kernel<<<(unsigned)ceil_div(heads, 64), 64, 0, st>>>(lp, runs, heads, glam);
     GATX_LAUNCH_CHECK("diff_attention_lam_join");
   }
   // B
@@ -1238,10 +1550,9 @@ extern "C" int gatx_diff_attention_backward(
     });
     GATX_LAUNCH_CHECK("diff_attention_gq");
     if (a.w.hub_blocks && gq) {
-      GATX_GRID(hub_bound * heads, "diff_attention_backward");
       with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
-        diff_grad_join_kernel<T><<<(unsigned)(hub_bound * heads), 256, 0, st>>>(a, (T*)gq, nullptr);
+        diff_sum_join_kernel<T><<<join_blocks(a.w, 1), 256, 0, st>>>(a, 1, (T*)gq, nullptr);
         return 0;
       });
       GATX_LAUNCH_CHECK("diff_attention_gq_join");
@@ -1275,11 +1586,9 @@ extern "C" int gatx_diff_attention_backward(
     });
     GATX_LAUNCH_CHECK("diff_attention_gkv");
     if (a.w.hub_blocks) {
-      GATX_GRID(src_hub_bound * heads, "diff_attention_backward");
       with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
-        diff_grad_join_kernel<T><<<(unsigned)(src_hub_bound * heads), 256, 0, st>>>(a, (T*)gk,
-                                                                                   (T*)gv);
+        diff_sum_join_kernel<T><<<join_blocks(a.w, 1), 256, 0, st>>>(a, 1, (T*)gk, (T*)gv);
         return 0;
       });
       GATX_LAUNCH_CHECK("diff_attention_gkv_join");

@@ -155,12 +155,16 @@ class DiffAttentionFunction(torch.autograd.Function):
         bias = None if bias is None else bias.contiguous()
         (qp, ldq), (kp, ldk), (vp, ldv) = _pack(dt, H, d, dv, q, k, v)
         out = torch.empty((M, H, dv), dtype=q.dtype, device=dev)
-        save = any(ctx.needs_input_grad[:5])
         E, N = graph.edge_bound, graph.num_nodes
-        S = torch.empty((H, max(E, 1), 2), dtype=torch.float32, device=dev) if save else None
-        stat = torch.empty((H, N, 4), dtype=torch.float32, device=dev) if save else None
-        hub = (0, None, None, 0) if nodes is not None else _hub_args(graph, False)
-        slots = M * pieces if nodes is not None and pieces > 1 else hub[3]
+        if nodes is None:
+            S = torch.empty((H, max(E, 1), 2), dtype=torch.float32, device=dev)
+            stat = torch.empty((H, N, 4), dtype=torch.float32, device=dev)
+            hub = _hub_args(graph, False)
+            slots = hub[3]
+        else:
+            S = stat = None
+            hub = (0, None, None, 0)
+            slots = M * pieces if pieces > 1 else 0
         nb = lib.gatx_diff_attention_part_bytes(slots, H, -(-dv // 8) * 8)
         part = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
         with _span("diff_attention", (M, E, H, d, dv)):
@@ -168,7 +172,7 @@ class DiffAttentionFunction(torch.autograd.Function):
                  ptr(graph.rowptr), ptr(graph.col), E, M, N, ptr(nodes), pieces, scale, ptr(lam),
                  ptr(bias), ptr(bucket), ptr(out), ptr(S), ptr(stat), *hub, ptr(part), nb,
                  stream())
-        if save:
+        if any(ctx.needs_input_grad[:5]):
             ctx.save_for_backward(qp, kp, vp, lam, bias, bucket, S, stat)
             ctx.graph, ctx.scale, ctx.lds, ctx.dims = graph, scale, (ldq, ldk, ldv), (H, d, dv)
         return out

@@ -201,18 +201,18 @@ def test_distill_c_refusals():
 def test_attention_c_refusals():
     #      dt q    ldq k    ldk v    ldv H  d  dv rowptr col E  M  N  nodes pieces
     ok = [0, ANY, 32, ANY, 32, ANY, 16, 2, 8, 8, ANY, ANY, 9, 6, 6, None, 1, 1.0, ANY, None, None,
-          ANY, None, None, 0, None, None, 0, None, 0, None]
+          ANY, ANY, ANY, 0, None, None, 0, None, 0, None]
     for at, value in ((0, 4), (1, None), (2, 31), (1, ANY + 4), (7, 0), (8, 257), (9, 513),
-                      (12, 1 << 31), (13, 5), (15, ANY), (19, ANY), (20, ANY), (21, None),
-                      (21, ANY + 8), (22, ANY), (24, 4)):
+                      (12, 1 << 31), (13, 5), (15, ANY), (16, 5000), (19, ANY), (20, ANY),
+                      (21, None), (21, ANY + 8), (22, None), (24, 4)):
         bad = list(ok)
         bad[at] = value
-        if at == 15:
-            bad[16] = 5000
+        if at == 16:
+            bad[15], bad[22], bad[23] = ANY, None, None
         rc, msg = c_call("gatx_diff_attention", *bad)
         assert rc == 1000 and "diff_attention" in msg, (at, msg)
     bad = list(ok)   # pieces without room for them
-    bad[15], bad[16] = ANY, 8
+    bad[15], bad[16], bad[22], bad[23] = ANY, 8, None, None
     rc, msg = c_call("gatx_diff_attention", *bad)
     assert rc == 1000 and "workspace" in msg
 
