@@ -21,7 +21,7 @@ namespace gatx {
 namespace {
 
 constexpr int kMaxCols = 8192;
-constexpr int kMaxParts = 1024;   // workgroups of the backward (their column partials)
+constexpr int kMaxParts = 768;    // workgroups of the backward (their column partials): 3 a CU
 
 struct NormArgs {
   const void *h, *resid, *gate, *gy, *gn;

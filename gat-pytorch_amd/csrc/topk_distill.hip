@@ -271,7 +271,8 @@ __global__ void __launch_bounds__(1024) distill_block_kernel(DistillArgs a) {
 }
 
 __global__ void __launch_bounds__(1024) distill_total_kernel(const float* part, int blocks,
-                                                             float* total) {
+                                                             float* total, int mean,
+                                                             float* count) {
   __shared__ float red[16];
   float l = 0.f, n = 0.f;
   for (int i = threadIdx.x; i < blocks; i += 1024) {
@@ -281,9 +282,8 @@ __global__ void __launch_bounds__(1024) distill_total_kernel(const float* part, 
   l = block_total(l, red);
   n = block_total(n, red);
   if (threadIdx.x == 0) {
-    total[0] = l;
-    total[1] = n;
-    total[2] = l / fmaxf(n, 1.f);
+    total[0] = mean ? l / fmaxf(n, 1.f) : l;
+    count[0] = n;
   }
 }
 
@@ -430,12 +430,16 @@ extern "C" size_t gatx_topk_distill_workspace_bytes(int64_t rows) {
 extern "C" int gatx_topk_distill(int dtype, const void* logits, int64_t rows, int64_t classes,
                                  int64_t ld, int teacher_dtype, const void* teacher,
                                  const void* index, int index_is_int64, int K, float temperature,
-                                 float* row_loss, float* total, float* stat, void* workspace,
-                                 size_t workspace_bytes, gatx_stream_t s) {
+                                 float* row_loss, float* total, int mean, float* count,
+                                 float* stat, void* workspace, size_t workspace_bytes, gatx_stream_t s) {
   GATX_CALL(check_distill("topk_distill", dtype, rows, classes, teacher_dtype, K, temperature));
   hipStream_t st = (hipStream_t)s;
+  GATX_REQUIRE(!total || count, "topk_distill: null count");
   if (rows == 0) {
-    if (total) zero_words_kernel<<<1, 64, 0, st>>>((uint32_t*)total, 3);
+    if (total) {
+      zero_words_kernel<<<1, 64, 0, st>>>((uint32_t*)total, 1);
+      zero_words_kernel<<<1, 64, 0, st>>>((uint32_t*)count, 1);
+    }
     GATX_LAUNCH_CHECK("topk_distill zero");
     return 0;
   }
@@ -457,7 +461,8 @@ extern "C" int gatx_topk_distill(int dtype, const void* logits, int64_t rows, in
   });
   GATX_LAUNCH_CHECK("topk_distill");
   if (total) {
-    distill_total_kernel<<<1, 1024, 0, st>>>((const float*)workspace, blocks, total);
+    distill_total_kernel<<<1, 1024, 0, st>>>((const float*)workspace, blocks, total, mean,
+                                            count);
     GATX_LAUNCH_CHECK("topk_distill_total");
   }
   return 0;

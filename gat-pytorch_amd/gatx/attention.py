@@ -17,7 +17,7 @@ from torch import nn
 from torch.autograd.function import once_differentiable
 
 from . import tuning
-from ._lib import DTYPES, call, lib, ptr, stream
+from ._lib import DTYPES, call, lib, on_device, ptr, stream
 from .functional import _span
 from .graph import Graph, graph_cache
 
@@ -185,7 +185,7 @@ class DiffAttentionFunction(torch.autograd.Function):
         N, E, dev, dtype = graph.num_nodes, graph.edge_bound, qp.device, qp.dtype
         dt = DTYPES[dtype]
         need_q, need_k, need_v, need_lam, need_bias = ctx.needs_input_grad[:5]
-        with torch.cuda.device(dev):
+        with on_device(dev):
             (gop, ldgo), = _pack(dt, H, d, dv, v=go)[2:]
             gq = torch.empty((N, H, 2, d), dtype=dtype, device=dev) if need_q else None
             gk = torch.empty((N, H, 2, d), dtype=dtype, device=dev) if need_k else None
@@ -283,7 +283,7 @@ def diff_attention(q, k, v, lam, graph: Graph, *, scale=None, bias=None, positio
         nodes = nodes.to(torch.int64).contiguous()
         items = max(1, nodes.numel() * q.size(1))
         pieces = max(1, min(_SERVING_WAVES // items, 256, -(-graph.edge_bound // 256)))
-    with torch.cuda.device(graph.device):
+    with on_device(graph.device):
         bucket = None
         if bias is not None:
             bucket = _buckets(graph, positions.contiguous(), bias.size(0), int(max_distance),

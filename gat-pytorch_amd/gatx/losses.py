@@ -10,7 +10,7 @@ from __future__ import annotations
 import torch
 from torch.autograd.function import once_differentiable
 
-from ._lib import DTYPES, call, lib, ptr, stream
+from ._lib import DTYPES, call, lib, on_device, ptr, stream
 from .functional import _span
 
 
@@ -98,35 +98,37 @@ class TopKDistillationFunction(torch.autograd.Function):
         teacher, index = teacher.contiguous(), index.contiguous()
         save = ctx.needs_input_grad[0]
         none = reduction == "none"
-        row_loss = torch.empty(n, device=dev) if none else None
-        total = None if none else torch.empty(3, device=dev)
-        stat = torch.empty((n, 4), device=dev) if save else None
+        loss = torch.empty(n if none else (), device=dev)
         wb = 0 if none else lib.gatx_topk_distill_workspace_bytes(n)
-        ws = torch.empty(wb, dtype=torch.uint8, device=dev) if wb else None
-        args = (DTYPES[x.dtype], ptr(x), n, C, ld, DTYPES[teacher.dtype], ptr(teacher),
-                ptr(index), int(index.dtype == torch.int64), K, temperature)
+        # the rows' statistics and their number, for the backward, and the workspace behind them
+        stat = torch.empty(16 * n + 16 + wb, dtype=torch.uint8, device=dev)
+        p, at = ptr(stat), ptr(stat) + 16 * n
+        row, total, count = (ptr(loss), None, None) if none else (None, ptr(loss), at)
         with _span("topk_distill", (n, C, K)):
-            call("gatx_topk_distill", *args, ptr(row_loss), ptr(total), ptr(stat), ptr(ws), wb,
+            call("gatx_topk_distill", DTYPES[x.dtype], ptr(x), n, C, ld, DTYPES[teacher.dtype],
+                 ptr(teacher), ptr(index), int(index.dtype == torch.int64), K, temperature, row,
+                 total, int(reduction == "mean"), count, p if save else None, at + 16, wb,
                  stream())
         if save:
-            ctx.save_for_backward(x, teacher, index, stat, total)
-            ctx.args, ctx.reduction = (ld, temperature), reduction
-        return row_loss if none else total[2] if reduction == "mean" else total[0]
+            ctx.save_for_backward(x, teacher, index, stat)
+            ctx.args = ld, temperature, reduction
+        return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        x, teacher, index, stat, total = ctx.saved_tensors
-        (ld, temperature), (n, C) = ctx.args, x.shape
-        with torch.cuda.device(x.device):
+        x, teacher, index, stat = ctx.saved_tensors
+        (ld, temperature, reduction), (n, C) = ctx.args, x.shape
+        with on_device(x.device):
             g = g.to(torch.float32).contiguous()
             grad = torch.empty((n, C), dtype=x.dtype, device=x.device)
-            count = ptr(total) + 4 if ctx.reduction == "mean" else None
+            p = ptr(stat)
             with _span("topk_distill_bwd", (n, C)):
                 call("gatx_topk_distill_backward", DTYPES[x.dtype], ptr(x), n, C, ld,
                      DTYPES[teacher.dtype], ptr(teacher), ptr(index),
-                     int(index.dtype == torch.int64), teacher.size(1), temperature, ptr(stat),
-                     ptr(g), int(ctx.reduction == "none"), count, ptr(grad), stream())
+                     int(index.dtype == torch.int64), teacher.size(1), temperature, p, ptr(g),
+                     int(reduction == "none"), p + 16 * n if reduction == "mean" else None,
+                     ptr(grad), stream())
         return grad, None, None, None, None
 
 
@@ -172,7 +174,7 @@ def topk_distillation(logits: torch.Tensor, teacher_logits: torch.Tensor,
                          "none")
     if not logits.is_cuda:
         raise RuntimeError("gatx: topk_distillation needs HIP tensors (no CPU path)")
-    with torch.cuda.device(logits.device):
+    with on_device(logits.device):
         return TopKDistillationFunction.apply(logits, teacher_logits, teacher_index, temperature,
                                               reduction)
 

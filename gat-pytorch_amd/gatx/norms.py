@@ -15,7 +15,7 @@ import torch
 from torch import nn
 from torch.autograd.function import once_differentiable
 
-from ._lib import DTYPES, call, lib, ptr, stream
+from ._lib import DTYPES, call, lib, on_device, ptr, stream
 from .functional import _span
 
 MAX_COLUMNS = 8192
@@ -70,7 +70,7 @@ class BlockNormFunction(torch.autograd.Function):
         (ldh, ldr, ldg), dev, dt = ctx.lds, h.device, DTYPES[h.dtype]
         n, D = h.shape
         need = ctx.needs_input_grad
-        with torch.cuda.device(dev):
+        with on_device(dev):
             (gy2, ldgy), (gn2, ldgn) = _opt(gy), _opt(gn)
 
             def rows(wanted):
@@ -129,7 +129,7 @@ def _f32(t):
 def norm_before(x, weight, eps: float = 1e-6):
     """weight * rms(x): the norm before a block. x: (..., D), weight: (D,)."""
     _check("norm_before", x, [("weight", weight)], [])
-    with torch.cuda.device(x.device):
+    with on_device(x.device):
         return BlockNormFunction.apply(x, None, None, None, None, _f32(weight), float(eps))[1]
 
 
@@ -148,7 +148,7 @@ def norm_after(h, weight, *, resid=None, gate=None, scale=None, next_weight=None
                        resid=None if resid is None else resid.unsqueeze(0),
                        gate=None if gate is None else gate.unsqueeze(0))
         return r.squeeze(0) if next_weight is None else tuple(t.squeeze(0) for t in r)
-    with torch.cuda.device(h.device):
+    with on_device(h.device):
         y, nxt = BlockNormFunction.apply(h, _f32(weight), resid,
                                          gate.float() if vector_gate else gate, _f32(scale),
                                          _f32(next_weight), float(eps))

@@ -709,16 +709,17 @@ int gatx_block_norm_backward(int dtype, int64_t rows, int64_t cols, const void* 
  * or int32; a slot of a negative class or of teacher -inf is empty): p = softmax over the row's
  * slots of t / T, q = softmax of s / T, loss_i = T^2 sum_k p_k (log p_k - log q[index_k]). A class
  * may come twice (its slots add up). A row without slots has loss 0 and no gradient; an index >=
- * classes makes its row NaN. row_loss (nullable): rows floats; total (nullable): {sum of the losses,
- * the number of rows with slots, sum / max(number, 1)}. stat (rows x 4, nullable, for the
- * backward): the maxima and the sums' logarithms (base 2) of both softmaxes. K <= 1024. workspace: gatx_topk_distill_workspace_bytes(). Fixed-order sums. */
+ * classes makes its row NaN. row_loss (nullable): rows floats; total (nullable): the sum of the losses,
+ * divided by max(count, 1) where `mean`, with *count = the number of rows with slots. stat (rows x
+ * 4, nullable, for the backward): the maxima and the sums' logarithms (base 2) of both softmaxes.
+ * K <= 1024. workspace: gatx_topk_distill_workspace_bytes(). Fixed-order sums. */
 size_t gatx_topk_distill_workspace_bytes(int64_t rows);
 int gatx_topk_distill(int dtype, const void* logits, int64_t rows, int64_t classes, int64_t ld,
                       int teacher_dtype, const void* teacher, const void* index,
-                      int index_is_int64, int K, float temperature, float* row_loss, float* total,
-                      float* stat, void* workspace, size_t workspace_bytes, gatx_stream_t stream);
+                      int index_is_int64, int K, float temperature, float* row_loss, float* total, int mean,
+                      float* count, float* stat, void* workspace, size_t workspace_bytes, gatx_stream_t stream);
 /* grad (rows x classes, packed, dtype) = g T (q - sum of p at each class), g = g[i * g_stride]
- * (g_stride 0 or 1) divided by max(*count, 1) when count is given (the forward's &total[1]). */
+ * (g_stride 0 or 1) divided by max(*count, 1) when count is given (the forward's). */
 int gatx_topk_distill_backward(int dtype, const void* logits, int64_t rows, int64_t classes,
                                int64_t ld, int teacher_dtype, const void* teacher,
                                const void* index, int index_is_int64, int K, float temperature,

@@ -183,9 +183,9 @@ def test_block_norm_backward_c_refusals():
 
 
 def test_distill_c_refusals():
-    ok = [0, ANY, 4, 8, 8, 0, ANY, ANY, 1, 2, 1.0, None, ANY, None, ANY, 10 ** 6, None]
+    ok = [0, ANY, 4, 8, 8, 0, ANY, ANY, 1, 2, 1.0, None, ANY, 1, ANY, None, ANY, 10 ** 6, None]
     for at, value in ((0, 5), (5, 9), (1, None), (2, -1), (3, 0), (9, 0), (9, 1025), (10, 0.0),
-                      (10, float("nan")), (10, float("inf")), (15, 4)):
+                      (10, float("nan")), (10, float("inf")), (14, None), (17, 4)):
         bad = list(ok)
         bad[at] = value
         rc, msg = c_call("gatx_topk_distill", *bad)

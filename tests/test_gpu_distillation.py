@@ -217,6 +217,18 @@ def test_same_bits_every_time_and_captured(C, device):
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), s
 
 
+def test_loss_scaled_in_place(device):
+    """The loss may be changed in place before its backward (gradient accumulation)."""
+    from gatx.losses import topk_distillation
+    x, t, i = make(30, 20, 4, torch.float32, device)
+    want = run(x, t, i, 1.0)[1] / 4
+    x.requires_grad_(True)
+    loss = topk_distillation(x, t, i)
+    loss /= 4
+    loss.backward()
+    assert torch.equal(x.grad, want)
+
+
 def test_no_rows(device):
     loss, g = run(torch.zeros(0, 9, device=device), torch.zeros(0, 2, device=device),
                   torch.zeros(0, 2, dtype=torch.int64, device=device), 1.0)
