@@ -60,18 +60,6 @@ __device__ inline Raw<float> load8<float>(const float* p) {
   return r;
 }
 template <typename T>
-__device__ inline Raw<T> zero8() {
-  Raw<T> r;
-  r.v = make_uint4(0, 0, 0, 0);
-  return r;
-}
-template <>
-__device__ inline Raw<float> zero8<float>() {
-  Raw<float> r;
-  r.a = r.b = make_float4(0, 0, 0, 0);
-  return r;
-}
-template <typename T>
 __device__ inline Raw<T> keep8(bool keep, Raw<T> x) {
   x.v.x = keep ? x.v.x : 0u;
   x.v.y = keep ? x.v.y : 0u;
@@ -403,7 +391,12 @@ struct Edge {
     j = it.n > 0 ? c : 0;
   }
 };
-constexpr int kFlight = 4;   // edges whose rows are in flight per slot
+// Edges whose rows are in flight per slot. Logits: 8 of the 16-bit types (PPI, bf16 d = 128 / fp16 d =
+// 64: 206 / 119 us, against 220 / 134 with 4), 4 of float32 (d = 61: 318 us, 373 with 8). The other
+// passes keep more waves with 2 (fp16: values 103 us, 112 with 4; dw 98 / 108; gq 118 / 128).
+template <typename T>
+constexpr int kDotFlight = sizeof(T) == 2 ? 8 : 4;
+constexpr int kFlight = 2;
 
 // One row's state over a slot's edges: both maps' running maximum and sum.
 template <int NV>
@@ -632,7 +625,7 @@ struct Tiles {
 // The logits of every edge and the softmax statistics of every row.
 template <typename T, int G, bool BIAS>
 __global__ void __launch_bounds__(256) diff_score_kernel(AttnArgs a) {
-  constexpr int NL = kTile<G>, U = NL < kFlight ? NL : kFlight;
+  constexpr int NL = kTile<G>, U = NL < kDotFlight<T> ? NL : kDotFlight<T>;
   const Item it = find_item(a.w);
   const Lane<G, 1> l(a.w.gs, a.dp, 8);
   const Tiles<G> tl(it, a.w.gs);
@@ -961,7 +954,7 @@ __global__ void __launch_bounds__(256) diff_gq_kernel(AttnArgs a) {
 // C: gk and gv of every source from its out-edges (CSR w.rowptr = srowptr, col = scol).
 template <typename T, int G, int NV>
 __global__ void __launch_bounds__(256) diff_gkv_kernel(AttnArgs a) {
-  constexpr int NL = kTile<G>, U = NL < 2 ? NL : 2;
+  constexpr int NL = kTile<G>, U = NL < kFlight ? NL : kFlight;
   const Item it = find_item(a.w);
   const Lane<G, NV> l(a.w.gs, a.dp, a.dvp);
   const Tiles<G> tl(it, a.w.gs);
@@ -1157,22 +1150,33 @@ __global__ void __launch_bounds__(256) relative_bucket_kernel(BucketArgs a) {
 struct PackArgs {
   const void* src[3];
   void* dst[3];
-  int64_t ld[3], n[3];   // n: 8-element chunks of the packed tensor
-  int groups[3], width[3];
+  int64_t ld[3], n[3];   // n: elements of the packed tensor
+  int groups[3], width[3], padded[3];
 };
+// One element a lane and turn: both sides are read and written in order, four rounds in flight.
+// (44 900 x 6 heads of d = 61, dv = 121 in float32: k and v in 102 us = 5.3 TB/s. Reading q unpacked
+// where it is needed, once a row, costs more than its share here: the logits 318 -> 395 us.)
 template <typename T>
 __global__ void __launch_bounds__(256) pack_heads_kernel(PackArgs a) {
+  constexpr int R = 4;
   const int t = blockIdx.y;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= a.n[t]) return;
-  const int w = a.width[t], chunks = (w + 7) / 8;
-  const int64_t g = i / chunks, row = g / a.groups[t];
-  const int c = (int)(i - g * chunks) * 8;
-  const T* s = (const T*)a.src[t] + row * a.ld[t] + (g - row * a.groups[t]) * w;
-  Pack<T, 8> x;
+  const uint32_t w = a.width[t], wp = a.padded[t], row_elems = wp * a.groups[t];
+  const int64_t i0 = (int64_t)blockIdx.x * (256 * R) + threadIdx.x;
+  if (i0 >= a.n[t]) return;
+  const T* src = (const T*)a.src[t];
+  T* dst = (T*)a.dst[t];
+  T x[R];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) x.v[j] = c + j < w ? s[c + j] : (T)0.f;
-  *reinterpret_cast<Pack<T, 8>*>((T*)a.dst[t] + i * 8) = x;
+  for (int r = 0; r < R; ++r) {
+    const int64_t i = i0 + r * 256;
+    const int64_t row = i / row_elems;
+    const uint32_t in = (uint32_t)(i - row * row_elems), g = in / wp, c = in - g * wp;
+    x[r] = (T)0.f;
+    if (i < a.n[t] && c < w) x[r] = src[row * a.ld[t] + g * w + c];
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+    if (i0 + r * 256 < a.n[t]) dst[i0 + r * 256] = x[r];
 }
 
 // ------------------------------------------------------------------ launches
@@ -1303,7 +1307,8 @@ extern "C" int gatx_diff_attention_pack(int dtype, int64_t rows, int64_t keys, i
   auto add = [&](const void* src, int64_t ld, void* dst, int64_t n, int groups, int width) {
     if (!src || n == 0) return;
     a.src[t] = src; a.dst[t] = dst; a.ld[t] = ld; a.groups[t] = groups; a.width[t] = width;
-    a.n[t] = n * groups * ceil_div(width, 8);
+    a.padded[t] = (int)round_up(width, 8);
+    a.n[t] = n * groups * a.padded[t];
     most = std::max(most, a.n[t]);
     ++t;
   };
@@ -1313,8 +1318,8 @@ extern "C" int gatx_diff_attention_pack(int dtype, int64_t rows, int64_t keys, i
   if (t == 0) return 0;
   for (int i = 0; i < t; ++i)
     GATX_REQUIRE(a.dst[i] && aligned16(a.dst[i]), "diff_attention_pack: bad destination");
-  GATX_GRID(ceil_div(most, 256), "diff_attention_pack");
-  const dim3 grid((unsigned)ceil_div(most, 256), t);
+  GATX_GRID(ceil_div(most, 1024), "diff_attention_pack");
+  const dim3 grid((unsigned)ceil_div(most, 1024), t);
   with_dtype(dtype, [&](auto x) {
     pack_heads_kernel<decltype(x)><<<grid, 256, 0, (hipStream_t)s>>>(a);
     return 0;

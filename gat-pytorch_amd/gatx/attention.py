@@ -186,7 +186,7 @@ class DiffAttentionFunction(torch.autograd.Function):
         dt = DTYPES[dtype]
         need_q, need_k, need_v, need_lam, need_bias = ctx.needs_input_grad[:5]
         with on_device(dev):
-            (gop, ldgo), = _pack(dt, H, d, dv, v=go)[2:]
+            gop, ldgo = _pack(dt, H, d, dv, v=go)[2]
             gq = torch.empty((N, H, 2, d), dtype=dtype, device=dev) if need_q else None
             gk = torch.empty((N, H, 2, d), dtype=dtype, device=dev) if need_k else None
             gv = torch.empty((N, H, dv), dtype=dtype, device=dev) if need_v else None

@@ -202,7 +202,7 @@ def test_attention_c_refusals():
     #      dt q    ldq k    ldk v    ldv H  d  dv rowptr col E  M  N  nodes pieces
     ok = [0, ANY, 32, ANY, 32, ANY, 16, 2, 8, 8, ANY, ANY, 9, 6, 6, None, 1, 1.0, ANY, None, None,
           ANY, ANY, ANY, 0, None, None, 0, None, 0, None]
-    for at, value in ((0, 4), (1, None), (2, 31), (1, ANY + 4), (7, 0), (8, 257), (9, 513),
+    for at, value in ((0, 4), (1, None), (2, 31), (1, ANY + 4), (4, 31), (7, 0), (8, 257), (9, 513),
                       (12, 1 << 31), (13, 5), (15, ANY), (16, 5000), (19, ANY), (20, ANY),
                       (21, None), (21, ANY + 8), (22, None), (24, 4)):
         bad = list(ok)
