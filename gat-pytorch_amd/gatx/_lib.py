@@ -184,7 +184,19 @@ def _load():
     return lib
 
 
+def _load_host():
+    """gatx._host (csrc/host.cpp): the autograd nodes of the graph-transformer operators. Loaded after
+    libgatx.so, which resolves its symbols."""
+    try:
+        from . import _host
+    except ImportError as e:
+        raise ImportError(f"gatx: the host module gatx/_host.so is missing or does not load ({e}); "
+                          "build it with `make -C gat-pytorch_amd/csrc`") from e
+    return _host
+
+
 lib = _load()
+host = _load_host()
 
 
 def check(rc: int, what: str = ""):

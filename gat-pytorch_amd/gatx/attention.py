@@ -14,11 +14,9 @@ import math
 
 import torch
 from torch import nn
-from torch.autograd.function import once_differentiable
 
 from . import tuning
-from ._lib import DTYPES, call, lib, on_device, ptr, stream
-from .functional import _span
+from ._lib import DTYPES, host as _host, on_device
 from .graph import Graph, graph_cache
 
 MAX_HEAD_WIDTH = 256    # d
@@ -61,70 +59,15 @@ def bucket_bounds(num_buckets: int, max_distance: int, bidirectional: bool):
 _BOUNDS: dict = {}
 
 
-def _bounds_array(num_buckets, max_distance, bidirectional):
-    """bucket_bounds as the host array of a launch (a pure function of its three numbers)."""
-    import ctypes
+def _bounds(num_buckets, max_distance, bidirectional):
+    """bucket_bounds, kept by its three numbers (the search is in whole numbers of any size)."""
     key = (num_buckets, max_distance, bidirectional)
     hit = _BOUNDS.get(key)
     if hit is None:
-        m, b = bucket_bounds(num_buckets, max_distance, bidirectional)
-        hit = _BOUNDS[key] = (m, (ctypes.c_int64 * max(len(b), 1))(*b), len(b))
+        hit = _BOUNDS[key] = bucket_bounds(num_buckets, max_distance, bidirectional)
         while len(_BOUNDS) > 64:
             _BOUNDS.pop(next(iter(_BOUNDS)))
     return hit
-
-
-def _buckets(graph: Graph, positions, num_buckets, max_distance, bidirectional, nodes):
-    import ctypes
-    m, bounds, n = _bounds_array(num_buckets, max_distance, bool(bidirectional))
-    bucket = torch.empty(max(graph.edge_bound, 1), dtype=torch.uint8, device=graph.device)
-    call("gatx_relative_buckets", ptr(graph.rowptr), ptr(graph.col), ptr(graph.rowidx),
-         graph.edge_bound, graph.num_nodes, ptr(nodes), 0 if nodes is None else nodes.numel(),
-         ptr(positions), int(positions.dtype == torch.int64), m,
-         ctypes.addressof(bounds), n, int(bool(bidirectional)), ptr(bucket), stream())
-    return bucket
-
-
-def _rows(t: torch.Tensor):
-    """(tensor, row stride) with each row's heads packed: the tensor itself where only its rows
-    are strided (a slice of a fused projection's output), else a packed copy."""
-    want = 1
-    for size, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
-        if size != 1 and stride != want:
-            t = t.contiguous()
-            return t, t.stride(0)
-        want *= size
-    return t, (t.stride(0) if t.size(0) > 1 else want)
-
-
-def _chunked(t, ld, width) -> bool:
-    """Whether the kernels read these rows as they are: 8-element chunks, 16-byte aligned."""
-    return width % 8 == 0 and t.data_ptr() % 16 == 0 and ld * t.element_size() % 16 == 0
-
-
-def _pack(dtype, H, d, dv, q=None, k=None, v=None):
-    """[(tensor, row stride)] of q, k, v (None: absent) in the kernels' layout, one launch for those
-    that are not yet."""
-    given = [None if t is None else _rows(t) for t in (q, k, v)]
-    out, args, any_packed = [], [], False
-    rows = keys = 0
-    for i, (pair, width, groups) in enumerate(zip(given, (d, d, dv), (2 * H, 2 * H, H))):
-        if pair is None or _chunked(*pair, width):
-            out.append(pair)
-            args += [None, 0, None]
-            continue
-        t, ld = pair
-        p = torch.empty((t.size(0), groups, -(-width // 8) * 8), dtype=t.dtype, device=t.device)
-        out.append((p, p.stride(0)))
-        args += [ptr(t), ld, ptr(p)]
-        any_packed = True
-        if i == 0:
-            rows = t.size(0)
-        else:
-            keys = t.size(0)
-    if any_packed:
-        call("gatx_diff_attention_pack", dtype, rows, keys, H, d, dv, *args, stream())
-    return out
 
 
 def _needs(graph: Graph, built: bool, what: str):
@@ -135,80 +78,16 @@ def _needs(graph: Graph, built: bool, what: str):
                            "once eagerly)")
 
 
-def _hub_args(graph: Graph, source: bool):
-    """(edges, plan, count, bound) of the pieces of long rows."""
+_NO_PLAN = (0, None, None, 0)
+
+
+def _hub_plan(graph: Graph, source: bool):
+    """(edges, entries, count, bound) of the pieces of long rows."""
     T = tuning.get("attn_hub_edges")
     if T <= 0 or graph.edge_bound <= T:
-        return 0, None, None, 0
+        return _NO_PLAN
     _needs(graph, (T, source) in graph._hub_plans, "hub plan")
-    hubs, count, bound = graph.hub_plan(T, source)
-    return T, ptr(hubs), ptr(count), bound
-
-
-class DiffAttentionFunction(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, lam, bias, graph: Graph, scale: float, bucket, nodes, pieces: int):
-        dt, dev = DTYPES[q.dtype], q.device
-        M, H, _, d = q.shape
-        dv = v.size(2)
-        lam = lam.contiguous()
-        bias = None if bias is None else bias.contiguous()
-        (qp, ldq), (kp, ldk), (vp, ldv) = _pack(dt, H, d, dv, q, k, v)
-        out = torch.empty((M, H, dv), dtype=q.dtype, device=dev)
-        E, N = graph.edge_bound, graph.num_nodes
-        if nodes is None:
-            S = torch.empty((H, max(E, 1), 2), dtype=torch.float32, device=dev)
-            stat = torch.empty((H, N, 4), dtype=torch.float32, device=dev)
-            hub = _hub_args(graph, False)
-            slots = hub[3]
-        else:
-            S = stat = None
-            hub = (0, None, None, 0)
-            slots = M * pieces if pieces > 1 else 0
-        nb = lib.gatx_diff_attention_part_bytes(slots, H, -(-dv // 8) * 8)
-        part = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
-        with _span("diff_attention", (M, E, H, d, dv)):
-            call("gatx_diff_attention", dt, ptr(qp), ldq, ptr(kp), ldk, ptr(vp), ldv, H, d, dv,
-                 ptr(graph.rowptr), ptr(graph.col), E, M, N, ptr(nodes), pieces, scale, ptr(lam),
-                 ptr(bias), ptr(bucket), ptr(out), ptr(S), ptr(stat), *hub, ptr(part), nb,
-                 stream())
-        if any(ctx.needs_input_grad[:5]):
-            ctx.save_for_backward(qp, kp, vp, lam, bias, bucket, S, stat)
-            ctx.graph, ctx.scale, ctx.lds, ctx.dims = graph, scale, (ldq, ldk, ldv), (H, d, dv)
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, go):
-        qp, kp, vp, lam, bias, bucket, S, stat = ctx.saved_tensors
-        graph, (H, d, dv), (ldq, ldk, ldv) = ctx.graph, ctx.dims, ctx.lds
-        N, E, dev, dtype = graph.num_nodes, graph.edge_bound, qp.device, qp.dtype
-        dt = DTYPES[dtype]
-        need_q, need_k, need_v, need_lam, need_bias = ctx.needs_input_grad[:5]
-        with on_device(dev):
-            gop, ldgo = _pack(dt, H, d, dv, v=go)[2]
-            gq = torch.empty((N, H, 2, d), dtype=dtype, device=dev) if need_q else None
-            gk = torch.empty((N, H, 2, d), dtype=dtype, device=dev) if need_k else None
-            gv = torch.empty((N, H, dv), dtype=dtype, device=dev) if need_v else None
-            glam = torch.empty(H, dtype=torch.float32, device=dev) if need_lam else None
-            nb = bias.size(0) if need_bias else 0
-            gbias = torch.empty((nb, H), dtype=torch.float32, device=dev) if need_bias else None
-            hub = _hub_args(graph, False)
-            src_hub, T = (None, None, 0), (None, None, None)
-            if need_k or need_v:
-                _needs(graph, graph.srowptr is not None, "transpose")
-                graph.ensure_transpose()
-                src_hub = _hub_args(graph, True)[1:]
-                T = (ptr(graph.srowptr), ptr(graph.scol), ptr(graph.seid))
-            wb = lib.gatx_diff_attention_backward_workspace_bytes(N, E, H, d, dv, nb, hub[3],
-                                                                  src_hub[2])
-            ws = torch.empty(wb, dtype=torch.uint8, device=dev)
-            with _span("diff_attention_bwd", (N, E, H, d, dv)):
-                call("gatx_diff_attention_backward", dt, ptr(qp), ldq, ptr(kp), ldk, ptr(vp), ldv,
-                     ptr(gop), ldgo, H, d, dv, ptr(graph.rowptr), ptr(graph.col), *T, E, N,
-                     ctx.scale, ptr(lam), ptr(bucket), nb, ptr(S), ptr(stat), ptr(gq), ptr(gk),
-                     ptr(gv), ptr(glam), ptr(gbias), *hub, *src_hub, ptr(ws), wb, stream())
-        return gq, gk, gv, glam, gbias, None, None, None, None, None
+    return (T, *graph.hub_plan(T, source))
 
 
 def _check(q, k, v, lam, graph, bias, positions, nodes):
@@ -274,23 +153,26 @@ def diff_attention(q, k, v, lam, graph: Graph, *, scale=None, bias=None, positio
     _check(q, k, v, lam, graph, bias, positions, nodes)
     graph.poll()
     scale = 1.0 / math.sqrt(q.size(3)) if scale is None else float(scale)
-    pieces = 1
+    exact, bounds = (0, []) if bias is None else _bounds(bias.size(0), int(max_distance),
+                                                         bool(bidirectional))
+    grad = torch.is_grad_enabled()
+    args = (q, k, v, lam, bias, positions, exact, bounds, bool(bidirectional), scale, graph.rowptr,
+            graph.col, graph.rowidx, graph.num_nodes, graph.edge_bound)
     if nodes is not None:
-        if torch.is_grad_enabled() and any(t is not None and t.requires_grad
-                                           for t in (q, k, v, lam, bias)):
+        if grad and any(t is not None and t.requires_grad for t in (q, k, v, lam, bias)):
             raise RuntimeError("gatx: diff_attention(nodes=...) has no gradients: call it under "
                                "torch.no_grad()")
-        nodes = nodes.to(torch.int64).contiguous()
         items = max(1, nodes.numel() * q.size(1))
         pieces = max(1, min(_SERVING_WAVES // items, 256, -(-graph.edge_bound // 256)))
-    with on_device(graph.device):
-        bucket = None
-        if bias is not None:
-            bucket = _buckets(graph, positions.contiguous(), bias.size(0), int(max_distance),
-                              bidirectional, nodes)
-        return DiffAttentionFunction.apply(
-            q, k, v, lam.float(), None if bias is None else bias.float(), graph, scale, bucket,
-            nodes, pieces)
+        return _host.diff_attention_nodes(*args, nodes, pieces)
+    with on_device(graph.device):   # (the graph's own launches)
+        transpose, src_plan = (None, None, None), _NO_PLAN
+        if grad and (k.requires_grad or v.requires_grad):
+            _needs(graph, graph.srowptr is not None, "transpose")
+            graph.ensure_transpose()
+            transpose = (graph.srowptr, graph.scol, graph.seid)
+            src_plan = _hub_plan(graph, True)
+        return _host.diff_attention(*args, _hub_plan(graph, False), *transpose, src_plan)
 
 
 class DiffAttention(nn.Module):

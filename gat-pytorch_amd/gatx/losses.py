@@ -8,9 +8,8 @@ And distillation from a teacher's top logits (csrc/topk_distill.hip)."""
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
-from ._lib import DTYPES, call, lib, on_device, ptr, stream
+from ._lib import call, host as _host, lib, ptr, stream
 from .functional import _span
 
 
@@ -85,53 +84,6 @@ class BCEWithLogitsLoss(torch.nn.Module):
         return BCEWithLogitsFunction.apply(input, target, self.pw)
 
 
-class TopKDistillationFunction(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, teacher, index, temperature: float, reduction: str):
-        dev = logits.device
-        n, C = logits.shape
-        K = teacher.size(1)
-        x = logits
-        if C > 1 and x.stride(1) != 1:
-            x = x.contiguous()
-        ld = x.stride(0) if n > 1 else C
-        teacher, index = teacher.contiguous(), index.contiguous()
-        save = ctx.needs_input_grad[0]
-        none = reduction == "none"
-        loss = torch.empty(n if none else (), device=dev)
-        wb = 0 if none else lib.gatx_topk_distill_workspace_bytes(n)
-        # the rows' statistics and their number, for the backward, and the workspace behind them
-        stat = torch.empty(16 * n + 16 + wb, dtype=torch.uint8, device=dev)
-        p, at = ptr(stat), ptr(stat) + 16 * n
-        row, total, count = (ptr(loss), None, None) if none else (None, ptr(loss), at)
-        with _span("topk_distill", (n, C, K)):
-            call("gatx_topk_distill", DTYPES[x.dtype], ptr(x), n, C, ld, DTYPES[teacher.dtype],
-                 ptr(teacher), ptr(index), int(index.dtype == torch.int64), K, temperature, row,
-                 total, int(reduction == "mean"), count, p if save else None, at + 16, wb,
-                 stream())
-        if save:
-            ctx.save_for_backward(x, teacher, index, stat)
-            ctx.args = ld, temperature, reduction
-        return loss
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g):
-        x, teacher, index, stat = ctx.saved_tensors
-        (ld, temperature, reduction), (n, C) = ctx.args, x.shape
-        with on_device(x.device):
-            g = g.to(torch.float32).contiguous()
-            grad = torch.empty((n, C), dtype=x.dtype, device=x.device)
-            p = ptr(stat)
-            with _span("topk_distill_bwd", (n, C)):
-                call("gatx_topk_distill_backward", DTYPES[x.dtype], ptr(x), n, C, ld,
-                     DTYPES[teacher.dtype], ptr(teacher), ptr(index),
-                     int(index.dtype == torch.int64), teacher.size(1), temperature, p, ptr(g),
-                     int(reduction == "none"), p + 16 * n if reduction == "mean" else None,
-                     ptr(grad), stream())
-        return grad, None, None, None, None
-
-
 def topk_distillation(logits: torch.Tensor, teacher_logits: torch.Tensor,
                       teacher_index: torch.Tensor, temperature: float = 1.0,
                       reduction: str = "mean") -> torch.Tensor:
@@ -143,40 +95,7 @@ def topk_distillation(logits: torch.Tensor, teacher_logits: torch.Tensor,
     teacher logit of -inf) is an empty slot; a class may come twice; one past the last makes its
     row NaN. A row without slots has loss 0 and no gradient. reduction "mean" is over the rows that
     have slots (0 if none has), "sum", or "none" (one float32 a row). Only logits get a gradient."""
-    for name, t in (("logits", logits), ("teacher_logits", teacher_logits),
-                    ("teacher_index", teacher_index)):
-        if t.device != logits.device:
-            raise RuntimeError(f"gatx: topk_distillation: {name} is on {t.device}, logits on "
-                               f"{logits.device}")
-        if t.dim() != 2:
-            raise ValueError(f"gatx: topk_distillation: {name} has two dimensions, got "
-                             f"{tuple(t.shape)}")
-    if logits.dtype not in DTYPES or teacher_logits.dtype not in DTYPES:
-        raise RuntimeError("gatx: topk_distillation takes float32, bfloat16 or float16 logits, got "
-                           f"{logits.dtype} and {teacher_logits.dtype}")
-    if teacher_index.dtype not in (torch.int64, torch.int32):
-        raise RuntimeError("gatx: topk_distillation: teacher_index must be int64 or int32, got "
-                           f"{teacher_index.dtype}")
-    if (teacher_logits.shape != teacher_index.shape or logits.size(0) != teacher_index.size(0)
-            or logits.size(1) < 1 or not 1 <= teacher_index.size(1) <= 1024):
-        raise ValueError("gatx: topk_distillation: (rows, classes) logits and (rows, K <= 1024) "
-                         f"teacher logits and classes, got {tuple(logits.shape)}, "
-                         f"{tuple(teacher_logits.shape)}, {tuple(teacher_index.shape)}")
-    if teacher_logits.requires_grad:
-        raise RuntimeError("gatx: topk_distillation does not differentiate the teacher; pass "
-                           "teacher_logits.detach()")
-    temperature = float(temperature)
-    if not 0.0 < temperature < float("inf"):
-        raise ValueError(f"gatx: topk_distillation: temperature must be positive, got "
-                         f"{temperature}")
-    if reduction not in ("mean", "sum", "none"):
-        raise ValueError(f"gatx: topk_distillation: reduction {reduction!r} is not mean, sum or "
-                         "none")
-    if not logits.is_cuda:
-        raise RuntimeError("gatx: topk_distillation needs HIP tensors (no CPU path)")
-    with on_device(logits.device):
-        return TopKDistillationFunction.apply(logits, teacher_logits, teacher_index, temperature,
-                                              reduction)
+    return _host.topk_distillation(logits, teacher_logits, teacher_index, temperature, reduction)
 
 
 class TopKDistillationLoss(torch.nn.Module):
