@@ -546,55 +546,55 @@ __global__ void __launch_bounds__(256) diff_serve_kernel(AttnArgs a) {
   }
 }
 
-// The pieces of a served row joined in order: a workgroup per (row, head), 4 runs of pieces side by
-// side.
+// The pieces of a served row joined: a workgroup per (row, head, 32 columns), both maps' sums in 16
+// runs of pieces side by side, each run and then the runs in order. (One node of 65 537 edges, 8
+// heads in 256 pieces: 14 us with a workgroup per (row, head).)
+constexpr int kJoinCols = 32, kJoinRuns = 16;
 template <typename T>
 __global__ void __launch_bounds__(1024) diff_serve_join_kernel(AttnArgs a) {
-  extern __shared__ __attribute__((aligned(16))) float lds[];   // [4][2 dvp]
-  const int64_t row = blockIdx.x / a.w.heads, first = row * a.w.pieces;
-  const int head = (int)(blockIdx.x - row * a.w.heads), pieces = a.w.pieces;
-  const int H = a.w.heads;
-  const float* p0 = a.part + (first * H + head) * a.part_width;
+  __shared__ float sums[kJoinRuns][2 * kJoinCols];
+  const int cb = (a.dv + kJoinCols - 1) / kJoinCols;
+  const int64_t rh = blockIdx.x / cb, row = rh / a.w.heads;
+  const int x0 = (int)(blockIdx.x - rh * cb) * kJoinCols;
+  const int head = (int)(rh - row * a.w.heads), pieces = a.w.pieces, H = a.w.heads;
+  const float* p0 = a.part + (row * pieces * H + head) * a.part_width;
   const int64_t step = (int64_t)H * a.part_width;
-  float m1 = -kInf, m2 = -kInf;
-  for (int i = threadIdx.x & 63; i < pieces; i += 64) {
-    m1 = fmaxf(m1, p0[i * step]);
-    m2 = fmaxf(m2, p0[i * step + 2]);
+  // every wave finds the maxima and sums for itself
+  const int lane = threadIdx.x & 63;
+  float m1 = -kInf, m2 = -kInf, l1 = 0.f, l2 = 0.f;
+  for (int i = lane; i < pieces; i += 64) {
+    const float4 s = *(const float4*)(p0 + i * step);
+    const float n1 = fmaxf(m1, s.x), n2 = fmaxf(m2, s.z);
+    const float r1 = finite_max(n1), r2 = finite_max(n2);
+    l1 = l1 * exp_(m1 - r1) + s.y * exp_(s.x - r1);
+    l2 = l2 * exp_(m2 - r2) + s.w * exp_(s.z - r2);
+    m1 = n1;
+    m2 = n2;
   }
-  for (int d = 1; d < 64; d <<= 1) {
-    m1 = fmaxf(m1, __shfl_xor(m1, d));
-    m2 = fmaxf(m2, __shfl_xor(m2, d));
-  }
-  const float r1 = finite_max(m1), r2 = finite_max(m2);
-  float l1 = 0.f, l2 = 0.f;
-  for (int i = threadIdx.x & 63; i < pieces; i += 64) {
-    l1 += p0[i * step + 1] * exp_(p0[i * step] - r1);
-    l2 += p0[i * step + 3] * exp_(p0[i * step + 2] - r2);
-  }
-  l1 = group_sum<64>(l1);
-  l2 = group_sum<64>(l2);
-  const int W = 2 * a.dvp, runs = 4, run = threadIdx.x >> 8, t = threadIdx.x & 255;
-  for (int x = t; x < W; x += 256) {
-    const bool second = x >= a.dvp;
-    const float r = second ? r2 : r1;
-    float s = 0.f;
+  const float t1 = slots_max<1>(m1, 64), t2 = slots_max<1>(m2, 64);
+  const float r1 = finite_max(t1), r2 = finite_max(t2);
+  l1 = group_sum<64>(l1 * exp_(m1 - r1));
+  l2 = group_sum<64>(l2 * exp_(m2 - r2));
+  // thread: column (lane & 31) of map (lane >> 5), run = its wave
+  const int run = threadIdx.x >> 6, x = x0 + (lane & 31), map = lane >> 5;
+  const float r = map ? r2 : r1;
+  float s = 0.f;
+  if (x < a.dv) {
+    const float* p = p0 + 4 + map * a.dvp + x;
 #pragma unroll 4
-    for (int i = run; i < pieces; i += runs)
-      s += p0[i * step + 4 + x] * exp_(p0[i * step + (second ? 2 : 0)] - r);
-    lds[run * W + x] = s;
+    for (int i = run; i < pieces; i += kJoinRuns)
+      s += p[i * step] * exp_(p0[i * step + 2 * map] - r);
   }
+  sums[run][lane] = s;
   __syncthreads();
-  const float i1 = l1 == 0.f ? 0.f : 1.f / l1, i2 = l2 == 0.f ? 0.f : 1.f / l2;
-  const float w2 = a.lam[head] * i2;
-  T* out = (T*)a.out + (row * H + head) * a.dv;
-  for (int x = threadIdx.x; x < a.dv; x += 1024) {
-    float s1 = 0.f, s2 = 0.f;
-    for (int k = 0; k < runs; ++k) {
-      s1 += lds[k * W + x];
-      s2 += lds[k * W + a.dvp + x];
-    }
-    out[x] = (T)(s1 * i1 - s2 * w2);
+  if (run != 0 || map != 0 || x >= a.dv) return;
+  float s1 = 0.f, s2 = 0.f;
+  for (int k = 0; k < kJoinRuns; ++k) {
+    s1 += sums[k][lane];
+    s2 += sums[k][kJoinCols + lane];
   }
+  const float i1 = l1 == 0.f ? 0.f : 1.f / l1, i2 = l2 == 0.f ? 0.f : 1.f / l2;
+  ((T*)a.out)[(row * H + head) * a.dv + x] = (T)(s1 * i1 - s2 * (a.lam[head] * i2));
 }
 
 // ------------------------------------------------------------------ forward over whole rows
@@ -1033,7 +1033,7 @@ __global__ void __launch_bounds__(256) diff_gkv_kernel(AttnArgs a) {
 // In float64: the rows' D_2 have both signs, and their sum is far smaller than they are together.
 constexpr int kLamRuns = 64;
 __global__ void __launch_bounds__(256) diff_lam_kernel(const float2* D, int64_t rows, int64_t per,
-                                                       double* part) {
+                                                       double* part, float* glam) {
   __shared__ double red[256];
   const int h = blockIdx.y;
   const int64_t r0 = blockIdx.x * per, r1 = min(rows, r0 + per);
@@ -1045,7 +1045,9 @@ __global__ void __launch_bounds__(256) diff_lam_kernel(const float2* D, int64_t 
     __syncthreads();
     if ((int)threadIdx.x < d) red[threadIdx.x] += red[threadIdx.x + d];
   }
-  if (threadIdx.x == 0) part[h * gridDim.x + blockIdx.x] = red[0];
+  if (threadIdx.x) return;
+  if (gridDim.x == 1) glam[h] = (float)-red[0];
+  else part[h * gridDim.x + blockIdx.x] = red[0];
 }
 __global__ void __launch_bounds__(64) diff_lam_join_kernel(const double* part, int runs, int heads,
                                                            float* glam) {
@@ -1363,7 +1365,7 @@ extern "C" int gatx_diff_attention(int dtype, const void* q, int64_t ldq, const 
   if (nodes) {
     GATX_REQUIRE(pieces >= 1 && pieces <= 4096, "diff_attention: 1..4096 pieces");
     const int64_t items = rows * heads * pieces;
-    GATX_GRID(items, "diff_attention");
+    GATX_GRID(std::max(items, rows * heads * ceil_div(dv, kJoinCols)), "diff_attention");
     GATX_REQUIRE(pieces == 1 || (part && part_bytes >= gatx_diff_attention_part_bytes(
                                              rows * pieces, heads, a.dvp)),
                  "diff_attention: workspace too small");
@@ -1386,7 +1388,7 @@ extern "C" int gatx_diff_attention(int dtype, const void* q, int64_t ldq, const 
     if (pieces > 1) {
       with_dtype(dtype, [&](auto t) {
         diff_serve_join_kernel<decltype(t)>
-            <<<(unsigned)(rows * heads), 1024, sizeof(float) * 8 * a.dvp, st>>>(a);
+            <<<(unsigned)(rows * heads * ceil_div(dv, kJoinCols)), 1024, 0, st>>>(a);
         return 0;
       });
       GATX_LAUNCH_CHECK("diff_attention_serve_join");
@@ -1538,10 +1540,12 @@ extern "C" int gatx_diff_attention_backward(
   if (glam) {
     const int runs = (int)std::min<int64_t>(kLamRuns, ceil_div(N, 1024));
     double* lp = (double*)(ws + l.lam);
-    diff_lam_kernel<<<dim3(runs, heads), 256, 0, st>>>(a.D, N, ceil_div(N, runs), lp);
+    diff_lam_kernel<<<dim3(runs, heads), 256, 0, st>>>(a.D, N, ceil_div(N, runs), lp, glam);
     GATX_LAUNCH_CHECK("diff_attention_lam");
-    diff_lam_join_kernel<<<(unsigned)ceil_div(heads, 64), 64, 0, st>>>(lp, runs, heads, glam);
-    GATX_LAUNCH_CHECK("diff_attention_lam_join");
+    if (runs > 1) {
+      diff_lam_join_kernel<<<(unsigned)ceil_div(heads, 64), 64, 0, st>>>(lp, runs, heads, glam);
+      GATX_LAUNCH_CHECK("diff_attention_lam_join");
+    }
   }
   // B
   if (gq || by_source || gbias) {

@@ -89,43 +89,63 @@ __device__ inline float lanes_most(float v, int lanes) {
   return v;
 }
 
-// One row's teacher: a lane's slots li, li + lanes, ...: the largest logit and whether any counts.
-__device__ inline float teacher_max(const DistillArgs& a, int64_t at, int li, int lanes, bool& bad) {
+// A slot: its class (-1: empty) and teacher logit. Both loads are issued at once and used later, so a
+// lane's first slot is on its way while the row's logits are.
+struct Slot {
+  int c = -1;
+  float t = -kInf;
+  __device__ Slot(const DistillArgs& a, int64_t at, int j) {
+    const int k = min(j, a.K - 1);
+    const int cls = class_at(a, at + k);
+    const float x = teacher_at(a, at + k);
+    if (j < a.K && cls >= 0 && x != -kInf) {
+      c = cls;
+      t = x;
+    }
+  }
+  __device__ bool there() const { return c >= 0; }
+  __device__ bool past() const { return c == 0x7fffffff; }
+};
+// f(slot) for a lane's slots li, li + lanes, ... that are not empty; `first` is slot li.
+template <typename F>
+__device__ inline void each_slot(const DistillArgs& a, const Slot& first, int64_t at, int li,
+                                 int lanes, F&& f) {
+  if (first.there()) f(first);
+  for (int j = li + lanes; j < a.K; j += lanes) {
+    const Slot s(a, at, j);
+    if (s.there()) f(s);
+  }
+}
+// One row's teacher: a lane's largest logit, and whether a slot is out of range or NaN.
+__device__ inline float teacher_max(const DistillArgs& a, const Slot& first, int64_t at, int li,
+                                    int lanes, bool& bad) {
   float tm = -kInf;
   bad = false;
-  for (int j = li; j < a.K; j += lanes) {
-    const int c = class_at(a, at + j);
-    if (c < 0) continue;
-    const float t = teacher_at(a, at + j);
-    if (t == -kInf) continue;
-    bad |= c == 0x7fffffff || t != t;
-    tm = fmaxf(tm, t);
-  }
+  each_slot(a, first, at, li, lanes, [&](const Slot& s) {
+    bad |= s.past() || s.t != s.t;
+    tm = fmaxf(tm, s.t);
+  });
   return tm;
 }
-__device__ inline float teacher_sum(const DistillArgs& a, int64_t at, int li, int lanes, float tm) {
+__device__ inline float teacher_sum(const DistillArgs& a, const Slot& first, int64_t at, int li,
+                                    int lanes, float tm) {
   float ts = 0.f;
-  for (int j = li; j < a.K; j += lanes) {
-    if (class_at(a, at + j) < 0) continue;
-    const float t = teacher_at(a, at + j);
-    if (t != -kInf) ts += __builtin_amdgcn_exp2f((t - tm) * a.k);
-  }
+  each_slot(a, first, at, li, lanes,
+            [&](const Slot& s) { ts += __builtin_amdgcn_exp2f((s.t - tm) * a.k); });
   return ts;
 }
 // Its share of sum_k p_k (log p_k - log q[c_k]), in units of ln 2: the logarithms are base 2.
 template <typename T>
-__device__ inline float slots_loss(const DistillArgs& a, const T* row, int64_t at, int li,
-                                   int lanes, float m, float ls, float tm, float lts) {
+__device__ inline float slots_loss(const DistillArgs& a, const T* row, const Slot& first,
+                                   int64_t at, int li, int lanes, float m, float ls, float tm,
+                                   float lts) {
   float sum = 0.f;
-  for (int j = li; j < a.K; j += lanes) {
-    const int c = class_at(a, at + j);
-    if (c < 0 || c == 0x7fffffff) continue;
-    const float t = teacher_at(a, at + j);
-    if (t == -kInf) continue;
-    const float lp = (t - tm) * a.k - lts, p = __builtin_amdgcn_exp2f(lp);
-    if (p > 0.f) sum += p * (lp - (((float)row[c] - m) * a.k - ls));
+  each_slot(a, first, at, li, lanes, [&](const Slot& s) {
+    if (s.past()) return;
+    const float lp = (s.t - tm) * a.k - lts, p = __builtin_amdgcn_exp2f(lp);
+    if (p > 0.f) sum += p * (lp - (((float)row[s.c] - m) * a.k - ls));
     else if (p != p) sum = p;
-  }
+  });
   return sum;
 }
 
@@ -140,24 +160,27 @@ __global__ void __launch_bounds__(256) distill_group_kernel(DistillArgs a) {
     if (r >= a.rows) continue;   // whole groups drop out; exchanges stay within a group
     const T* row = (const T*)a.logits + r * a.ld;
     const int64_t at = r * a.K;
+    const Slot slot(a, at, li);
     Lse z;
     for (int c = li; c < a.classes; c += 4 * lanes) {
       float x[4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) x[u] = c + u * lanes < a.classes ? (float)row[c + u * lanes] : -kInf;
+      for (int u = 0; u < 4; ++u) x[u] = (float)row[min(c + u * lanes, a.classes - 1)];
+#pragma unroll
+      for (int u = 1; u < 4; ++u) x[u] = c + u * lanes < a.classes ? x[u] : -kInf;
       lse_add(z, x, a.k);
     }
     lse_join_lanes(z, lanes, a.k);
     bool bad;
-    float tm = teacher_max(a, at, li, lanes, bad);
+    float tm = teacher_max(a, slot, at, li, lanes, bad);
     tm = lanes_most(tm, lanes);
     const bool any_bad = lanes_most(bad ? 1.f : 0.f, lanes) > 0.f;
     const bool has = tm != -kInf || any_bad;
-    const float ts = lanes_total(teacher_sum(a, at, li, lanes, tm), lanes);
+    const float ts = lanes_total(teacher_sum(a, slot, at, li, lanes, tm), lanes);
     const float ls = __builtin_amdgcn_logf(z.s), lts = __builtin_amdgcn_logf(ts);
     float loss = 0.f;
     if (has) {
-      loss = lanes_total(slots_loss(a, row, at, li, lanes, z.m, ls, tm, lts), lanes);
+      loss = lanes_total(slots_loss(a, row, slot, at, li, lanes, z.m, ls, tm, lts), lanes);
       loss = any_bad ? __builtin_nanf("") : loss * (a.T * a.T * kLn2);
     }
     if (li == 0) {
@@ -209,6 +232,7 @@ __global__ void __launch_bounds__(1024) distill_block_kernel(DistillArgs a) {
     const int64_t at = r * a.K;
     const int head = unaligned_head(row, a.classes);
     const int chunks = (a.classes - head) / V, tail = head + chunks * V;
+    const Slot slot(a, at, tid);
     Lse z;
     {
       float x[1] = {-kInf};
@@ -234,7 +258,7 @@ __global__ void __launch_bounds__(1024) distill_block_kernel(DistillArgs a) {
     }
     lse_join_lanes(z, 64, a.k);
     bool bad;
-    float tm = lanes_most(teacher_max(a, at, tid, nt, bad), 64);
+    float tm = lanes_most(teacher_max(a, slot, at, tid, nt, bad), 64);
     const float nbad = block_total(bad ? 1.f : 0.f, red);   // its barriers: the last
                                                             // row's readers of red_m, red_s, red_t
     if ((tid & 63) == 0) {
@@ -250,10 +274,10 @@ __global__ void __launch_bounds__(1024) distill_block_kernel(DistillArgs a) {
       tm = fmaxf(tm, red_t[i]);
     }
     const bool has = tm != -kInf || nbad > 0.f;
-    const float ts = block_total(teacher_sum(a, at, tid, nt, tm), red);
+    const float ts = block_total(teacher_sum(a, slot, at, tid, nt, tm), red);
     const float ls = __builtin_amdgcn_logf(z.s), lts = __builtin_amdgcn_logf(ts);
     float loss = block_total(
-        has ? slots_loss(a, row, at, tid, nt, z.m, ls, tm, lts) : 0.f, red);
+        has ? slots_loss(a, row, slot, at, tid, nt, z.m, ls, tm, lts) : 0.f, red);
     loss = nbad > 0.f ? __builtin_nanf("") : loss * (a.T * a.T * kLn2);
     if (tid == 0) {
       if (a.row_loss) a.row_loss[r] = loss;
@@ -287,21 +311,16 @@ __global__ void __launch_bounds__(1024) distill_total_kernel(const float* part, 
 }
 
 // The row's slots in LDS: class (-1: empty) and p. Returns whether a class is out of range.
-__device__ inline bool stage_slots(const DistillArgs& a, int64_t at, int li, int lanes, float tm,
-                                   float lts, int* cls, float* ps) {
+__device__ inline bool stage_slots(const DistillArgs& a, const Slot& first, int64_t at, int li,
+                                   int lanes, float tm, float lts, int* cls, float* ps) {
   bool bad = false;
-  for (int j = li; j < a.K; j += lanes) {
-    int c = class_at(a, at + j);
-    float p = 0.f;
-    if (c >= 0) {
-      const float t = teacher_at(a, at + j);
-      if (t == -kInf) c = -1;
-      else p = __builtin_amdgcn_exp2f((t - tm) * a.k - lts);
-      bad |= c == 0x7fffffff;
-    }
-    cls[j] = c == 0x7fffffff ? -1 : c;
-    ps[j] = p;
-  }
+  auto put = [&](int j, const Slot& s) {
+    bad |= s.past();
+    cls[j] = s.past() ? -1 : s.c;
+    ps[j] = s.there() ? __builtin_amdgcn_exp2f((s.t - tm) * a.k - lts) : 0.f;
+  };
+  if (li < a.K) put(li, first);
+  for (int j = li + lanes; j < a.K; j += lanes) put(j, Slot(a, at, j));
   return bad;
 }
 // The taught classes' gradients: the first slot of a class adds up all of its slots.
@@ -340,14 +359,23 @@ __global__ void __launch_bounds__(256) distill_group_grad_kernel(DistillArgs a) 
     if (r >= a.rows) continue;
     const T* row = (const T*)a.logits + r * a.ld;
     T* grad = (T*)a.grad + r * a.classes;
+    const Slot slot(a, r * a.K, li);
+    float x[4];   // the first turn's logits, on their way before anything waits
+#pragma unroll
+    for (int u = 0; u < 4; ++u) x[u] = (float)row[min(li + u * lanes, a.classes - 1)];
     const float4 st = *(const float4*)(a.stat + 4 * r);
     const bool has = st.w != -kInf;
     float gi = row_factor(a, r);
     bool bad = st.w != st.w;
-    if (has) bad |= stage_slots(a, r * a.K, li, lanes, st.z, st.w, cls, ps);
+    if (has) bad |= stage_slots(a, slot, r * a.K, li, lanes, st.z, st.w, cls, ps);
     if (lanes_most(bad ? 1.f : 0.f, lanes) > 0.f) gi = __builtin_nanf("");
-    for (int c = li; c < a.classes; c += lanes)
-      grad[c] = (T)(has ? gi * __builtin_amdgcn_exp2f(((float)row[c] - st.x) * a.k - st.y) : 0.f);
+    auto value = [&](float v) {
+      return (T)(has ? gi * __builtin_amdgcn_exp2f((v - st.x) * a.k - st.y) : 0.f);
+    };
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (li + u * lanes < a.classes) grad[li + u * lanes] = value(x[u]);
+    for (int c = li + 4 * lanes; c < a.classes; c += lanes) grad[c] = value((float)row[c]);
     wave_lds_sync();   // the slots and the stores above, before this wave's next ones
     if (has) write_slots(a, row, grad, li, lanes, gi, st.x, st.y, cls, ps);
     wave_lds_sync();
@@ -367,9 +395,10 @@ __global__ void __launch_bounds__(1024) distill_block_grad_kernel(DistillArgs a)
     const float4 st = *(const float4*)(a.stat + 4 * r);
     const bool has = st.w != -kInf;
     float gi = row_factor(a, r);
+    const Slot slot(a, r * a.K, tid);
     __syncthreads();   // the last row's readers of the slots
     bool bad = st.w != st.w;
-    if (has) bad |= stage_slots(a, r * a.K, tid, nt, st.z, st.w, cls, ps);
+    if (has) bad |= stage_slots(a, slot, r * a.K, tid, nt, st.z, st.w, cls, ps);
     if (block_total(bad ? 1.f : 0.f, red) > 0.f) gi = __builtin_nanf("");
     auto value = [&](float x) {
       return has ? gi * __builtin_amdgcn_exp2f((x - st.x) * a.k - st.y) : 0.f;

@@ -82,12 +82,33 @@ _NO_PLAN = (0, None, None, 0)
 
 
 def _hub_plan(graph: Graph, source: bool):
-    """(edges, entries, count, bound) of the pieces of long rows."""
+    """(edges, entries, count, bound) of the pieces of long rows; no plan once it is known that the
+    graph has none (its count is copied to the host when the plan is built and looked at when it
+    has arrived, so nothing waits; until then, and inside a first capture, the pieces' launches
+    find nothing to do)."""
     T = tuning.get("attn_hub_edges")
     if T <= 0 or graph.edge_bound <= T:
         return _NO_PLAN
-    _needs(graph, (T, source) in graph._hub_plans, "hub plan")
-    return (T, *graph.hub_plan(T, source))
+    plans, key = graph._hub_plans, (T, source, "entries")
+    known = plans.get(key)
+    if known == 0:
+        return _NO_PLAN
+    _needs(graph, (T, source) in plans, "hub plan")
+    hubs, count, bound = graph.hub_plan(T, source)
+    if not torch.cuda.is_current_stream_capturing():
+        if known is None:
+            # a graph built inside a capture has its counts only after a replay: never read
+            if graph._event is not None:
+                host = torch.empty(1, dtype=torch.int32, pin_memory=True)
+                host.copy_(count, non_blocking=True)
+                event = torch.cuda.Event()
+                event.record()
+                plans[key] = (host, event)
+        elif not isinstance(known, int) and known[1].query():
+            plans[key] = int(known[0])
+            if plans[key] == 0:
+                return _NO_PLAN
+    return T, hubs, count, bound
 
 
 def _check(q, k, v, lam, graph, bias, positions, nodes):
