@@ -44,7 +44,13 @@ class GATModel(nn.Module):
     def __init__(self, num_classes: int, num_input_node_features: int, num_layers: int,
                  num_heads_per_layer: List[int], heads_concat_per_layer: List[bool],
                  head_output_features_per_layer: List[int], add_skip_connection: List[bool],
-                 dropout: float, const_attention: bool = False, **kwargs):
+                 dropout: float, const_attention: bool = False, block_norm: bool = False,
+                 **kwargs):
+        """The reference's arguments (`models/GATModel.py:21-62`) and block_norm: norms around every
+        layer (gatx.norms). Each layer then reads the normed stream, and each hidden layer's
+        ELU output is normed, gated and scaled into the stream beside its skip (skip + scale
+        sigmoid(gate) weight rms(out); without a skip it replaces the stream), the next layer's
+        norm in the same pass; the last layer's output is the reference's."""
         super().__init__()
         self.num_layers = num_layers
         self.dropout = dropout
@@ -70,6 +76,13 @@ class GATModel(nn.Module):
                                    else nn.Linear(fin, skip_out, bias=False))
         self.gat_layer_list = nn.ModuleList(gat_layers)
         self.skip_layer_list = nn.ModuleList(skip_layers)
+        self.block_norm = block_norm
+        if block_norm:
+            from .norms import BlockNorm
+            self.input_norm_weight = nn.Parameter(torch.ones(gat_layers[0].in_features))
+            self.block_norm_list = nn.ModuleList(BlockNorm(
+                lay.num_heads * lay.out_features if lay.concat else lay.out_features)
+                for lay in gat_layers[:-1])
         # True: skip / ELU / dropout fused into the layers (gatx's wiring). False: the
         # reference's own forward (`models/GATModel.py:120-151`) op for op around gatx GATLayers —
         # exactly what the INTEGRATION.md §1 drop-in (swap the import) runs; bench.py
@@ -131,7 +144,38 @@ class GATModel(nn.Module):
                 x = F.elu(x)
         return x, edge_index, attention_weights_list
 
+    def _run_block_norm(self, x, edge_index, with_attention):
+        """The stack with norms around its layers (block_norm)."""
+        from .functional import input_dropout
+        from .norms import norm_before
+        if torch.compiler.is_compiling():
+            raise RuntimeError("gatx: block_norm is not supported under torch.compile")
+        attention_weights_list = []
+        skip_count, last = 0, len(self.gat_layer_list) - 1
+        normed = norm_before(x, self.input_norm_weight)
+        for i, layer in enumerate(self.gat_layer_list):
+            if self.training and self.dropout > 0:
+                normed = input_dropout(normed, self.dropout, torch.randint(
+                    0, 2 ** 62, (1,), dtype=torch.int64, device=x.device))
+            resid = None
+            if self.add_skip_connection[i]:
+                resid = self._resid(i, skip_count, x)
+                skip_count += 1
+            # the last layer's skip rides in its epilogue, as without norms
+            out = layer(normed, edge_index, return_attention_weights=with_attention,
+                        resid=resid if i == last else None, elu=i != last)
+            if with_attention:
+                out, (edge_index, att) = out
+                attention_weights_list.append(att)
+            if i == last:
+                x = out
+            else:
+                x, normed = self.block_norm_list[i](out, resid)
+        return x, edge_index, attention_weights_list
+
     def _run(self, x, edge_index, with_attention):
+        if self.block_norm:
+            return self._run_block_norm(x, edge_index, with_attention)
         if not self.fuse_wiring:
             return self._run_reference_wiring(x, edge_index, with_attention)
         attention_weights_list = []
