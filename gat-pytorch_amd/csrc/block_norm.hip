@@ -24,7 +24,8 @@ constexpr int kMaxCols = 8192;
 // Workgroups of the backward (their column partials): 3 a CU are what the registers of 16 elements of
 // five streams leave. 44 900 x 1024 bf16: 194 us with 768, 254 with 512, 255 with 1024 (a second
 // round for a quarter of them), 200 with 1536; 128 registers (4 a CU) spill: 344 us; the next row's
-// loads in flight as well cost the waves they need: 262 us. A copy of the same bytes takes 144 us.
+// loads in flight as well, or keeping a row unwidened between its two sums, cost the waves they need:
+// 262 and 277 us. A copy of the same bytes takes 144 us.
 constexpr int kMaxParts = 768;
 
 struct NormArgs {
@@ -429,7 +430,8 @@ extern "C" int gatx_block_norm(int dtype, int64_t rows, int64_t cols, const void
       {gate, weight, scale, next_weight, y, next}));
   a.lanes = g.lanes;
   const int64_t blocks = ceil_div(rows, g.rows_per_block());
-  GATX_REQUIRE(blocks < (1ll << 31), "block_norm: too many rows");
+  // a launch holds fewer than 2^32 threads (taking turns in a loop costs every call 4%)
+  GATX_REQUIRE(blocks * (g.block() ? g.lanes : 256) < (1ll << 32), "block_norm: too many rows");
   run_norm(dtype, a, g, false, blocks, (hipStream_t)s);
   GATX_LAUNCH_CHECK("block_norm");
   return 0;

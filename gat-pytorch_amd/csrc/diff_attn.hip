@@ -1263,8 +1263,9 @@ bool chunked(int dtype, const void* p, int64_t ld) {
 unsigned join_blocks(const Work& w, int per) {
   return (unsigned)std::min<int64_t>(ceil_div((int64_t)w.hub_bound * w.heads, per), 1024);
 }
-#define GATX_GRID(blocks, what)                                                             \
-  GATX_REQUIRE((blocks) < (1ll << 31), "%s: too many work items for one launch", what)
+// A launch holds fewer than 2^32 threads.
+#define GATX_GRID(blocks, threads, what)                                                    \
+  GATX_REQUIRE((blocks) * (threads) < (1ll << 32), "%s: too many work items for one launch", what)
 
 }  // namespace
 }  // namespace gatx
@@ -1320,7 +1321,7 @@ extern "C" int gatx_diff_attention_pack(int dtype, int64_t rows, int64_t keys, i
   if (t == 0) return 0;
   for (int i = 0; i < t; ++i)
     GATX_REQUIRE(a.dst[i] && aligned16(a.dst[i]), "diff_attention_pack: bad destination");
-  GATX_GRID(ceil_div(most, 1024), "diff_attention_pack");
+  GATX_GRID(ceil_div(most, 1024), 256, "diff_attention_pack");
   const dim3 grid((unsigned)ceil_div(most, 1024), t);
   with_dtype(dtype, [&](auto x) {
     pack_heads_kernel<decltype(x)><<<grid, 256, 0, (hipStream_t)s>>>(a);
@@ -1365,7 +1366,7 @@ extern "C" int gatx_diff_attention(int dtype, const void* q, int64_t ldq, const 
   if (nodes) {
     GATX_REQUIRE(pieces >= 1 && pieces <= 4096, "diff_attention: 1..4096 pieces");
     const int64_t items = rows * heads * pieces;
-    GATX_GRID(std::max(items, rows * heads * ceil_div(dv, kJoinCols)), "diff_attention");
+    GATX_REQUIRE(items < (1ll << 31), "diff_attention: too many rows and pieces");
     GATX_REQUIRE(pieces == 1 || (part && part_bytes >= gatx_diff_attention_part_bytes(
                                              rows * pieces, heads, a.dvp)),
                  "diff_attention: workspace too small");
@@ -1374,21 +1375,23 @@ extern "C" int gatx_diff_attention(int dtype, const void* q, int64_t ldq, const 
     a.w.nodes = nodes; a.w.pieces = pieces;
     a.w.gs = pieces > 1 ? 64 : row_lanes(g.G, items);
     a.w.gs_log = log2i(a.w.gs);
-    const unsigned blocks = (unsigned)ceil_div(items, 256 / a.w.gs);
+    const int64_t blocks = ceil_div(items, 256 / a.w.gs);
+    const int64_t joins = pieces > 1 ? rows * heads * ceil_div(dv, kJoinCols) : 0;
+    GATX_GRID(blocks, 256, "diff_attention");
+    GATX_GRID(joins, 1024, "diff_attention");
     with_dtype(dtype, [&](auto t) {
       using T = decltype(t);
       with_geom(g, [&](auto G, auto NV) {
         constexpr int kG = decltype(G)::value, kNV = decltype(NV)::value;
-        if (bias) diff_serve_kernel<T, kG, kNV, true><<<blocks, 256, 0, st>>>(a);
-        else diff_serve_kernel<T, kG, kNV, false><<<blocks, 256, 0, st>>>(a);
+        if (bias) diff_serve_kernel<T, kG, kNV, true><<<(unsigned)blocks, 256, 0, st>>>(a);
+        else diff_serve_kernel<T, kG, kNV, false><<<(unsigned)blocks, 256, 0, st>>>(a);
       });
       return 0;
     });
     GATX_LAUNCH_CHECK("diff_attention_serve");
     if (pieces > 1) {
       with_dtype(dtype, [&](auto t) {
-        diff_serve_join_kernel<decltype(t)>
-            <<<(unsigned)(rows * heads * ceil_div(dv, kJoinCols)), 1024, 0, st>>>(a);
+        diff_serve_join_kernel<decltype(t)><<<(unsigned)joins, 1024, 0, st>>>(a);
         return 0;
       });
       GATX_LAUNCH_CHECK("diff_attention_serve_join");
@@ -1398,7 +1401,7 @@ extern "C" int gatx_diff_attention(int dtype, const void* q, int64_t ldq, const 
   GATX_REQUIRE(hub_edges == 0 || (hubs && hub_count), "diff_attention: null hub plan");
   const int64_t blocks = plan_rows(a.w, rows, heads, row_lanes(g.G, rows * heads), rowptr,
                                    hub_edges, hubs, hub_count, hub_bound);
-  GATX_GRID(blocks, "diff_attention");
+  GATX_GRID(blocks, 256, "diff_attention");
   GATX_REQUIRE(a.w.hub_blocks == 0 ||
                    (part && part_bytes >= gatx_diff_attention_part_bytes(hub_bound, heads, a.dvp)),
                "diff_attention: workspace too small");
@@ -1523,7 +1526,7 @@ extern "C" int gatx_diff_attention_backward(
   const int gs = row_lanes(g.G, N * heads);
   // A
   int64_t blocks = plan_rows(a.w, N, heads, gs, rowptr, hub_edges, hubs, hub_count, hub_bound);
-  GATX_GRID(blocks, "diff_attention_backward");
+  GATX_GRID(blocks, 256, "diff_attention_backward");
   with_dtype(dtype, [&](auto t) {
     using T = decltype(t);
     with_geom(g, [&](auto G, auto NV) {
@@ -1584,7 +1587,7 @@ extern "C" int gatx_diff_attention_backward(
     a.part_width = 2 * dp + dvp;
     blocks = plan_rows(a.w, N, heads, gs, srowptr, hub_edges, src_hubs, src_hub_count,
                        src_hub_bound);
-    GATX_GRID(blocks, "diff_attention_backward");
+    GATX_GRID(blocks, 256, "diff_attention_backward");
     with_dtype(dtype, [&](auto t) {
       using T = decltype(t);
       with_geom(g, [&](auto G, auto NV) {

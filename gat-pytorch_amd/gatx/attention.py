@@ -16,7 +16,7 @@ import torch
 from torch import nn
 
 from . import tuning
-from ._lib import DTYPES, host as _host, on_device
+from ._lib import DTYPES, host as _host, on_device, stream
 from .graph import Graph, graph_cache
 
 MAX_HEAD_WIDTH = 256    # d
@@ -78,6 +78,28 @@ def _needs(graph: Graph, built: bool, what: str):
                            "once eagerly)")
 
 
+def _ready(graph: Graph, key, built: bool):
+    """What the graph builds on first use may be used next on another stream: that one waits for
+    the build. (A capture begins after the device has caught up.)"""
+    if torch.cuda.is_current_stream_capturing():
+        return
+    now, done = stream(), graph._hub_plans.get((key, "built"))
+    if built:
+        event = torch.cuda.Event()
+        event.record()
+        graph._hub_plans[(key, "built")] = (now, event)
+    elif done is not None and done[0] != now:
+        torch.cuda.current_stream().wait_event(done[1])
+
+
+def _transpose(graph: Graph):
+    missing = graph.srowptr is None
+    _needs(graph, not missing, "transpose")
+    graph.ensure_transpose()
+    _ready(graph, "transpose", missing)
+    return graph.srowptr, graph.scol, graph.seid
+
+
 _NO_PLAN = (0, None, None, 0)
 
 
@@ -93,8 +115,10 @@ def _hub_plan(graph: Graph, source: bool):
     known = plans.get(key)
     if known == 0:
         return _NO_PLAN
-    _needs(graph, (T, source) in plans, "hub plan")
+    missing = (T, source) not in plans
+    _needs(graph, not missing, "hub plan")
     hubs, count, bound = graph.hub_plan(T, source)
+    _ready(graph, (T, source), missing)
     if not torch.cuda.is_current_stream_capturing():
         if known is None:
             # a graph built inside a capture has its counts only after a replay: never read
@@ -189,9 +213,7 @@ def diff_attention(q, k, v, lam, graph: Graph, *, scale=None, bias=None, positio
     with on_device(graph.device):   # (the graph's own launches)
         transpose, src_plan = (None, None, None), _NO_PLAN
         if grad and (k.requires_grad or v.requires_grad):
-            _needs(graph, graph.srowptr is not None, "transpose")
-            graph.ensure_transpose()
-            transpose = (graph.srowptr, graph.scol, graph.seid)
+            transpose = _transpose(graph)
             src_plan = _hub_plan(graph, True)
         return _host.diff_attention(*args, _hub_plan(graph, False), *transpose, src_plan)
 
