@@ -135,7 +135,8 @@ __device__ inline void axpy8(float p, const Raw<T>& x, float (&acc)[8]) {
   unpack8(x, f);
   axpy8(p, f, acc);
 }
-// Columns [at, at + 8) of a packed row of `width` elements.
+// Columns [at, at + 8) of a packed row of `width` elements; !whole: rows that are aligned to an
+// element only and can end inside the 8.
 template <typename T>
 __device__ inline void store8(T* row, int at, int width, bool whole, const float (&x)[8]) {
   if (whole) {
@@ -146,6 +147,11 @@ __device__ inline void store8(T* row, int at, int width, bool whole, const float
     } else {
       store_f32<T, 8>(row + at, x);
     }
+  } else if (at + 8 <= width) {
+    T y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = (T)x[i];
+    __builtin_memcpy(row + at, y, sizeof(y));   // global stores need no alignment
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -1155,30 +1161,35 @@ struct PackArgs {
   int64_t ld[3], n[3];   // n: elements of the packed tensor
   int groups[3], width[3], padded[3];
 };
-// One element a lane and turn: both sides are read and written in order, four rounds in flight.
-// (44 900 x 6 heads of d = 61, dv = 121 in float32: k and v in 102 us = 5.3 TB/s. Reading q unpacked
-// where it is needed, once a row, costs more than its share here: the logits 318 -> 395 us.)
+// Four bytes of the packed side a lane and round, four rounds in flight: both sides are read and
+// written in order. (44 900 x 6 heads of d = 61, dv = 121 in float32: k and v in 102 us = 5.3 TB/s.
+// Reading q unpacked where it is needed, once a row, costs more than its share here: the logits
+// 318 -> 395 us.)
 template <typename T>
 __global__ void __launch_bounds__(256) pack_heads_kernel(PackArgs a) {
-  constexpr int R = 4;
+  constexpr int R = 4, V = 4 / sizeof(T);
   const int t = blockIdx.y;
   const uint32_t w = a.width[t], wp = a.padded[t], row_elems = wp * a.groups[t];
-  const int64_t i0 = (int64_t)blockIdx.x * (256 * R) + threadIdx.x;
+  const int64_t i0 = ((int64_t)blockIdx.x * (256 * R) + threadIdx.x) * V;
   if (i0 >= a.n[t]) return;
   const T* src = (const T*)a.src[t];
   T* dst = (T*)a.dst[t];
-  T x[R];
+  Pack<T, V> x[R];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const int64_t i = i0 + r * 256;
-    const int64_t row = i / row_elems;
+    const int64_t i = min(i0 + r * 256 * V, a.n[t] - V), row = i / row_elems;
     const uint32_t in = (uint32_t)(i - row * row_elems), g = in / wp, c = in - g * wp;
-    x[r] = (T)0.f;
-    if (i < a.n[t] && c < w) x[r] = src[row * a.ld[t] + g * w + c];
+    const T* p = src + row * a.ld[t] + g * w;
+#pragma unroll
+    for (uint32_t v = 0; v < V; ++v) x[r].v[v] = p[min(c + v, w - 1)];
+#pragma unroll
+    for (uint32_t v = 0; v < V; ++v) x[r].v[v] = c + v < w ? x[r].v[v] : (T)0.f;
   }
 #pragma unroll
-  for (int r = 0; r < R; ++r)
-    if (i0 + r * 256 < a.n[t]) dst[i0 + r * 256] = x[r];
+  for (int r = 0; r < R; ++r) {
+    const int64_t i = i0 + r * 256 * V;
+    if (i < a.n[t]) *(Pack<T, V>*)(dst + i) = x[r];
+  }
 }
 
 // ------------------------------------------------------------------ launches
@@ -1321,8 +1332,9 @@ extern "C" int gatx_diff_attention_pack(int dtype, int64_t rows, int64_t keys, i
   if (t == 0) return 0;
   for (int i = 0; i < t; ++i)
     GATX_REQUIRE(a.dst[i] && aligned16(a.dst[i]), "diff_attention_pack: bad destination");
-  GATX_GRID(ceil_div(most, 1024), 256, "diff_attention_pack");
-  const dim3 grid((unsigned)ceil_div(most, 1024), t);
+  const int64_t blocks = ceil_div(most * dtype_size(dtype), 4096);
+  GATX_GRID(blocks, 256, "diff_attention_pack");
+  const dim3 grid((unsigned)blocks, t);
   with_dtype(dtype, [&](auto x) {
     pack_heads_kernel<decltype(x)><<<grid, 256, 0, (hipStream_t)s>>>(a);
     return 0;
