@@ -7,6 +7,7 @@
 #include <torch/extension.h>
 
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
@@ -52,6 +53,29 @@ variable_list once(variable_list&& grads, const char* what) {
   torch::autograd::DelayedError error(std::string("gatx: ") + what + " has no second derivative",
                                       (int64_t)out.size());
   return error.apply(std::move(out));
+}
+
+// Forward-mode derivatives would be dropped without a word.
+template <typename... In>
+void no_tangents(const char* what, const In&... inputs) {
+  for (const Tensor* t : {&inputs...})
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), "gatx: ", what,
+                                " has no forward-mode derivative");
+}
+
+// A captured backward into a leaf that an eager graph on the default stream still holds would make
+// that stream, which cannot take part in a capture, wait for the captured one: the capture breaks
+// on the engine's thread, where nothing can be caught.
+void check_capture(const Node& node, const char* what) {
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+  for (const auto& edge : node.next_edges()) {
+    if (!edge.function || edge.function->num_outputs() != 0) continue;
+    const auto stream = edge.function->stream();
+    TORCH_CHECK(!stream || stream->id() != 0, "gatx: ", what,   // (0: the default stream)
+                ": the captured backward reaches a leaf of an autograd graph that is alive on the "
+                "default stream; drop that graph's results, or run the eager steps on the capture's "
+                "stream");
+  }
 }
 
 template <typename N, typename... In>
@@ -113,6 +137,7 @@ struct BlockNormBackward : public Node {
   }
   variable_list apply(variable_list&& go) override {
     std::lock_guard<std::mutex> lock(mutex_);
+    check_capture(*this, "block norm");
     const Tensor x = h.unpack(), w = weight.unpack(), r = resid.unpack(), g = gate.unpack(),
                  sc = scale.unpack(), nw = next_weight.unpack();
     variable_list out(6);
@@ -154,6 +179,7 @@ struct BlockNormBackward : public Node {
 std::pair<Tensor, Tensor> block_norm(const Tensor& h, Tensor weight, const Tensor& resid, Tensor gate,
                                      Tensor scale, Tensor next_weight, bool gate_rows, double eps) {
   const c10::DeviceGuard guard(h.device());
+  no_tangents("block norm", h, weight, resid, gate, scale, next_weight);
   weight = f32(weight);
   scale = f32(scale);
   next_weight = f32(next_weight);
@@ -245,6 +271,7 @@ struct Distill {
 
 variable_list TopKDistillationBackward::apply(variable_list&& go) {
   std::lock_guard<std::mutex> lock(mutex_);
+  check_capture(*this, "topk_distillation");
   const Tensor x = logits.unpack(), t = teacher.unpack(), i = index.unpack();
   variable_list out(1);
   if (!go[0].defined()) return out;
@@ -285,12 +312,14 @@ Tensor topk_distillation(const Tensor& logits, const Tensor& teacher, const Tens
                     "got ", logits.sizes(), ", ", teacher.sizes(), ", ", index.sizes());
   TORCH_CHECK(!teacher.requires_grad(), me, " does not differentiate the teacher; pass "
               "teacher_logits.detach()");
-  TORCH_CHECK_VALUE(temperature > 0 && std::isfinite(temperature), me,
-                    ": temperature must be positive, got ", temperature);
+  // (T^2 and 1 / T stay float32 numbers)
+  TORCH_CHECK_VALUE(temperature >= 1e-18 && temperature <= 1e18, me,
+                    ": temperature must be positive (1e-18 to 1e18), got ", temperature);
   TORCH_CHECK_VALUE(reduction == "mean" || reduction == "sum" || reduction == "none", me,
                     ": reduction '", reduction, "' is not mean, sum or none");
   TORCH_CHECK(logits.is_cuda(), me, " needs HIP tensors (no CPU path)");
   const c10::DeviceGuard guard(logits.device());
+  no_tangents("topk_distillation", logits, teacher);
   const bool grad = torch::autograd::compute_requires_grad(logits), none = reduction == "none";
   Tensor loss, stat;
   {
@@ -405,6 +434,7 @@ struct DiffAttentionBackward : public Node {
   }
   variable_list apply(variable_list&& go) override {
     std::lock_guard<std::mutex> lock(mutex_);
+    check_capture(*this, "diff_attention");
     // (unpack also checks that nothing was changed in place since the forward)
     const Tensor qt = q.unpack(), kt = k.unpack(), vt = v.unpack(), lt = lam.unpack(),
                  bt = bias.unpack();
@@ -467,6 +497,7 @@ Tensor diff_attention(const Tensor& q, const Tensor& k, const Tensor& v, const T
                       const Opt& scol, const Opt& seid, const Plan& src_plan) {
   const c10::DeviceGuard guard(q.device());
   const Tensor lam = f32(lam_), bias = f32(of(bias_));
+  no_tangents("diff_attention", q, k, v, lam, bias);
   const bool grad = torch::autograd::compute_requires_grad(q, k, v, lam, bias);
   const int H = (int)q.size(1), d = (int)q.size(3), dv = (int)v.size(2);
   const Csr csr{rowptr, col, rowidx, num_nodes, edges};
@@ -523,8 +554,9 @@ Tensor diff_attention_nodes(const Tensor& q, const Tensor& k, const Tensor& v, c
                             int64_t num_nodes, int64_t edges, const Tensor& nodes_, int64_t pieces) {
   const c10::DeviceGuard guard(q.device());
   at::NoGradGuard no_grad;
-  const Tensor lam = f32(lam_).contiguous(), bias = packed(f32(of(bias_))),
-               nodes = nodes_.to(at::kLong).contiguous();
+  const Tensor lam = f32(lam_).contiguous(), bias = packed(f32(of(bias_)));
+  no_tangents("diff_attention", q, k, v, lam, bias);
+  const Tensor nodes = nodes_.to(at::kLong).contiguous();
   const int H = (int)q.size(1), d = (int)q.size(3), dv = (int)v.size(2);
   const int64_t M = nodes.numel();
   const Csr csr{rowptr, col, rowidx, num_nodes, edges};

@@ -452,7 +452,8 @@ int check_distill(const char* what, int dtype, int64_t rows, int64_t classes, in
   GATX_REQUIRE(rows >= 0 && classes >= 1 && classes < (1ll << 30), "%s: %lld x %lld logits", what,
                (long long)rows, (long long)classes);
   GATX_REQUIRE(K >= 1 && K <= kMaxSlots, "%s: %d slots a row (1..%d)", what, K, kMaxSlots);
-  GATX_REQUIRE(temperature > 0.f && temperature < kInf, "%s: temperature must be positive", what);
+  GATX_REQUIRE(temperature > 9e-19f && temperature < 1.1e18f,   // T^2 and 1 / T are float32 numbers
+               "%s: temperature must be positive (1e-18 to 1e18)", what);
   return 0;
 }
 

@@ -94,7 +94,8 @@ def topk_distillation(logits: torch.Tensor, teacher_logits: torch.Tensor,
     teacher_index (rows, K) int64 or int32: the slots' classes, K <= 1024. A negative class (or a
     teacher logit of -inf) is an empty slot; a class may come twice; one past the last makes its
     row NaN. A row without slots has loss 0 and no gradient. reduction "mean" is over the rows that
-    have slots (0 if none has), "sum", or "none" (one float32 a row). Only logits get a gradient."""
+    have slots (0 if none has), "sum", or "none" (one float32 a row). temperature: 1e-18 to 1e18. Only
+    logits get a gradient."""
     return _host.topk_distillation(logits, teacher_logits, teacher_index, temperature, reduction)
 
 

@@ -147,6 +147,14 @@ def test_distillation_arguments(change, error):
         TopKDistillationLoss(2.0)(torch.zeros(3, 8), torch.zeros(3, 2), torch.zeros(3, 2).long())
 
 
+@pytest.mark.parametrize("temperature", [-1.0, 1e-19, 1e19, float("inf"), 1e-60])
+def test_distillation_temperatures(temperature):
+    from gatx.losses import topk_distillation
+    with pytest.raises(ValueError, match="temperature"):
+        topk_distillation(torch.zeros(3, 8), torch.zeros(3, 2), torch.zeros(3, 2).long(),
+                          temperature)
+
+
 def c_call(name, *args):
     from gatx._lib import lib
     rc = getattr(lib, name)(*args)

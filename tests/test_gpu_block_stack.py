@@ -241,3 +241,82 @@ def test_training_step_captured_beside_an_eager_graph(device):
     for (n, a), b in zip(net.named_parameters(), twin.parameters()):
         assert torch.equal(a, b), n
     assert torch.isfinite(alive)
+
+
+def leaf_calls(device):
+    """{operator: (leaf, a call on it)}"""
+    from gatx import diff_attention, norm_after, norm_before
+    from gatx.graph import Graph
+    from gatx.losses import topk_distillation
+    N = 40
+    graph = Graph(torch.randint(0, N, (2, 300), device=device), N, False)
+    q, k = (torch.randn(N, 2, 2, 8, device=device) for _ in range(2))
+    v, lam = torch.randn(N, 2, 16, device=device), torch.rand(2, device=device)
+    h, w = torch.randn(N, 24, device=device), torch.ones(24, device=device)
+    t = torch.randn(N, 3, device=device)
+    i = torch.randint(0, 24, (N, 3), device=device)
+    return {"diff_attention": (q, lambda x: diff_attention(x, k, v, lam, graph)),
+            "norm_before": (h, lambda x: norm_before(x, w)),
+            "norm_after": (h, lambda x: norm_after(x, w, resid=h)),
+            "topk_distillation": (h, lambda x: topk_distillation(x, t, i))}
+
+
+OPERATORS = ["diff_attention", "norm_before", "norm_after", "topk_distillation"]
+
+
+@pytest.mark.parametrize("name", OPERATORS)
+def test_captured_backward_beside_an_eager_graph_on_the_default_stream(name, device):
+    """Refused while the eager graph of the same leaf lives; captured and right once it is gone."""
+    leaf, call = leaf_calls(device)[name]
+    x = leaf.clone().requires_grad_(True)
+    alive = call(x)
+    ones = torch.ones_like(alive)
+    want, = torch.autograd.grad(alive, x, ones, retain_graph=True)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+
+    def step():
+        return torch.autograd.grad(call(x), x, ones)[0]
+    with torch.cuda.stream(s):
+        torch.randn(4, device=device, requires_grad=True).sum().backward()   # the engine's thread
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="alive on the default stream"):
+        with torch.cuda.graph(graph, stream=s):
+            step()
+    torch.cuda.synchronize()
+    del alive
+    with torch.cuda.stream(s):
+        assert torch.equal(step(), want)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        got = step()
+    for _ in range(3):
+        got.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("name", OPERATORS)
+def test_forward_mode_is_refused(name, device):
+    import torch.autograd.forward_ad as fw
+    leaf, call = leaf_calls(device)[name]
+    with fw.dual_level():
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            call(fw.make_dual(leaf, torch.ones_like(leaf)))
+
+
+@pytest.mark.parametrize("name", OPERATORS)
+def test_a_second_backward_through_freed_inputs_is_refused(name, device):
+    leaf, call = leaf_calls(device)[name]
+    x = leaf.clone().requires_grad_(True)
+    loss = call(x).sum()
+    loss.backward(retain_graph=True)
+    first = x.grad.clone()
+    loss.backward()
+    assert torch.equal(x.grad, first + first)
+    with pytest.raises(RuntimeError, match="second time"):
+        loss.backward()
