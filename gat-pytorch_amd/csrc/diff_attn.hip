@@ -343,6 +343,7 @@ struct AttnArgs {
   Work w;
   const void *q, *k, *v, *go;
   int64_t ldq, ldk, ldv, ldgo;
+  int64_t q_end;             // elements of an unpacked q; 0: packed
   int d, dv, dp, dvp;
   const int32_t* col;        // (C: scol)
   const int32_t* seid;       // C
@@ -382,6 +383,29 @@ struct Lane {
     }
   }
 };
+// Chunk `at` of map m of a row of q. Unpacked rows (d as it is, any alignment) are read once a row
+// anyway, as whole unaligned chunks whose elements past d are dropped; a chunk that would pass the
+// end of q, element by element. (44 900 x 6 heads of d = 61 in float32: packing 160 -> 100 us, the logits 335 ->
+// 353.)
+template <typename T>
+__device__ inline Raw<T> load_q(const AttnArgs& a, int64_t row, int head, int m, int at) {
+  if (a.q_end == 0)
+    return load8((const T*)a.q + row * a.ldq + (int64_t)(2 * head + m) * a.dp + at);
+  const int64_t o = row * a.ldq + (int64_t)(2 * head + m) * a.d + at;
+  const T* p = (const T*)a.q + o;
+  T x[8];
+  if (o + 8 <= a.q_end) {
+    __builtin_memcpy(x, p, sizeof(x));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = at + i < a.d ? x[i] : (T)0.f;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = at + i < a.d ? p[i] : (T)0.f;
+  }
+  Raw<T> r;
+  __builtin_memcpy(&r, x, sizeof(r));
+  return r;
+}
 // Turns of `step` edges that cover the longest of the wave's rows.
 __device__ inline int turns_of(int n, int step) { return (n + step - 1) / step; }
 // Edge number o of an item. Past its end: its first edge again (index 0 of every array where it has
@@ -478,8 +502,7 @@ __global__ void __launch_bounds__(256) diff_serve_kernel(AttnArgs a) {
   const Lane<G, NV> l(a.w.gs, a.dp, a.dvp);
   const bool has = it.row >= 0;
   const int64_t row = has ? it.row : 0;
-  const T* qr = (const T*)a.q + row * a.ldq + (int64_t)it.head * 2 * a.dp + l.at_d;
-  const Raw<T> q1 = load8(qr), q2 = load8(qr + a.dp);
+  const Raw<T> q1 = load_q<T>(a, row, it.head, 0, l.at_d), q2 = load_q<T>(a, row, it.head, 1, l.at_d);
   Acc<NV> acc;
   const T* kb = (const T*)a.k + (int64_t)it.head * 2 * a.dp + l.at_d;
   const T* vb = (const T*)a.v + (int64_t)it.head * a.dvp;
@@ -637,8 +660,7 @@ __global__ void __launch_bounds__(256) diff_score_kernel(AttnArgs a) {
   const Tiles<G> tl(it, a.w.gs);
   const bool has = it.row >= 0;
   const int64_t row = has ? it.row : 0;
-  const T* qr = (const T*)a.q + row * a.ldq + (int64_t)it.head * 2 * a.dp + l.at_d;
-  const Raw<T> q1 = load8(qr), q2 = load8(qr + a.dp);
+  const Raw<T> q1 = load_q<T>(a, row, it.head, 0, l.at_d), q2 = load_q<T>(a, row, it.head, 1, l.at_d);
   const T* kb = (const T*)a.k + (int64_t)it.head * 2 * a.dp + l.at_d;
   const int64_t he = (int64_t)it.head * a.E;
   float m1 = -kInf, m2 = -kInf, s1 = 0.f, s2 = 0.f;
@@ -1162,9 +1184,7 @@ struct PackArgs {
   int groups[3], width[3], padded[3];
 };
 // Four bytes of the packed side a lane and round, four rounds in flight: both sides are read and
-// written in order. (44 900 x 6 heads of d = 61, dv = 121 in float32: k and v in 102 us = 5.3 TB/s.
-// Reading q unpacked where it is needed, once a row, costs more than its share here: the logits
-// 318 -> 395 us.)
+// written in order. (44 900 x 6 heads of d = 61, dv = 121 in float32: k and v in 100 us = 5.3 TB/s.)
 template <typename T>
 __global__ void __launch_bounds__(256) pack_heads_kernel(PackArgs a) {
   constexpr int R = 4, V = 4 / sizeof(T);
@@ -1356,12 +1376,15 @@ extern "C" int gatx_diff_attention(int dtype, const void* q, int64_t ldq, const 
                                    int hub_edges, const int32_t* hubs, const int32_t* hub_count,
                                    int64_t hub_bound, void* part, size_t part_bytes,
                                    gatx_stream_t s) {
+  const bool plain_q = dtype >= 0 && (dtype & GATX_Q_UNPACKED);
+  if (plain_q) dtype &= ~GATX_Q_UNPACKED;
   GATX_CALL(check_dims("diff_attention", dtype, heads, d, dv, E, std::max(rows, num_nodes)));
   if (rows == 0) return 0;
   GATX_REQUIRE(q && k && v && rowptr && col && lam && out, "diff_attention: null buffer");
   GATX_REQUIRE(nodes || rows == num_nodes, "diff_attention: a row for every node without nodes");
   GATX_REQUIRE(num_nodes > 0, "diff_attention: no nodes");
-  GATX_REQUIRE(chunked(dtype, q, ldq) && chunked(dtype, k, ldk) && chunked(dtype, v, ldv),
+  GATX_REQUIRE((plain_q ? ldq >= 0 : chunked(dtype, q, ldq)) && chunked(dtype, k, ldk) &&
+                   chunked(dtype, v, ldv),
                "diff_attention: rows of q, k, v must be 16-byte aligned (pack them)");
   GATX_REQUIRE(aligned16(out), "diff_attention: out must be 16-byte aligned");
   GATX_REQUIRE(!bias == !bucket, "diff_attention: bias and bucket go together");
@@ -1369,6 +1392,7 @@ extern "C" int gatx_diff_attention(int dtype, const void* q, int64_t ldq, const 
                "diff_attention: S and stat hold whole rows' logits (not with nodes)");
   AttnArgs a = {};
   a.q = q; a.k = k; a.v = v; a.ldq = ldq; a.ldk = ldk; a.ldv = ldv;
+  a.q_end = plain_q ? (rows - 1) * ldq + (int64_t)2 * heads * d : 0;
   a.d = d; a.dv = dv; a.dp = (int)round_up(d, 8); a.dvp = (int)round_up(dv, 8);
   a.col = col; a.E = E; a.scale = scale; a.lam = lam; a.bias = bias; a.bucket = bucket;
   a.S = (float2*)S; a.stat = (float4*)stat; a.out = out;

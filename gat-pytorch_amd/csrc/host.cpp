@@ -398,6 +398,15 @@ std::array<Rows, 3> chunked(const Tensor& q, const Tensor& k, const Tensor& v, i
   return out;
 }
 
+// The same where nothing is gathered from q later: its rows stay as they are. *dtype gets the flag.
+std::array<Rows, 3> chunked_keys(const Tensor& q, const Tensor& k, const Tensor& v, int H, int d,
+                                 int dv, int* dtype) {
+  std::array<Rows, 3> out = chunked({}, k, v, H, d, dv);
+  out[0] = heads_of(q);
+  *dtype |= GATX_Q_UNPACKED;
+  return out;
+}
+
 // A graph's CSR (gatx.Graph) as the calls need it.
 struct Csr {
   Tensor rowptr, col, rowidx;
@@ -508,13 +517,14 @@ Tensor diff_attention(const Tensor& q, const Tensor& k, const Tensor& v, const T
     at::NoGradGuard no_grad;
     if (bias.defined())
       bucket = relative_buckets(csr, *positions_, exact, bounds, bidirectional, {});
-    rows = chunked(q, k, v, H, d, dv);
+    int dtype = code(q.scalar_type());
+    rows = grad ? chunked(q, k, v, H, d, dv) : chunked_keys(q, k, v, H, d, dv, &dtype);
     out = at::empty({num_nodes, H, dv}, q.options());
     S = floats(q, {H, std::max<int64_t>(edges, 1), 2});
     stat = floats(q, {H, num_nodes, 4});
     const size_t pb = gatx_diff_attention_part_bytes(hubs.bound, H, (dv + 7) / 8 * 8);
     const Tensor part = bytes(q, pb), lp = packed(lam), bp = packed(bias);
-    run(gatx_diff_attention(code(q.scalar_type()), ptr(rows[0].t), rows[0].ld, ptr(rows[1].t),
+    run(gatx_diff_attention(dtype, ptr(rows[0].t), rows[0].ld, ptr(rows[1].t),
                             rows[1].ld, ptr(rows[2].t), rows[2].ld, H, d, dv, ints(rowptr),
                             ints(col), edges, num_nodes, num_nodes, nullptr, 1, (float)scale,
                             fptr(lp), fptr(bp), (const uint8_t*)ptr(bucket), ptr(out), fptr(S),
@@ -563,11 +573,12 @@ Tensor diff_attention_nodes(const Tensor& q, const Tensor& k, const Tensor& v, c
   Tensor bucket;
   if (bias.defined())
     bucket = relative_buckets(csr, *positions_, exact, bounds, bidirectional, nodes);
-  const auto rows = chunked(q, k, v, H, d, dv);
+  int dtype = code(q.scalar_type());
+  const auto rows = chunked_keys(q, k, v, H, d, dv, &dtype);
   const Tensor out = at::empty({M, H, dv}, q.options());
   const size_t pb = gatx_diff_attention_part_bytes(pieces > 1 ? M * pieces : 0, H, (dv + 7) / 8 * 8);
   const Tensor part = bytes(q, pb);
-  run(gatx_diff_attention(code(q.scalar_type()), ptr(rows[0].t), rows[0].ld, ptr(rows[1].t),
+  run(gatx_diff_attention(dtype, ptr(rows[0].t), rows[0].ld, ptr(rows[1].t),
                           rows[1].ld, ptr(rows[2].t), rows[2].ld, H, d, dv, ints(rowptr), ints(col),
                           edges, M, num_nodes, (const int64_t*)ptr(nodes), (int)pieces,
                           (float)scale, fptr(lam), fptr(bias), (const uint8_t*)ptr(bucket), ptr(out),

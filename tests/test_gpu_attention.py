@@ -371,3 +371,28 @@ def test_second_derivative_is_refused(device):
     gq, = torch.autograd.grad(out.square().sum(), q, create_graph=True)
     with pytest.raises(RuntimeError):
         gq.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("N", [1, 2, 5, 70])
+@pytest.mark.parametrize("H,d,dv", [(1, 1, 1), (3, 7, 5), (2, 8, 16), (1, 9, 8), (3, 61, 121),
+                                    (1, 250, 3)])
+def test_queries_read_where_they_are(H, d, dv, N, dtype, device):
+    """Without gradients q is not repacked: rows of any width and alignment up to the last element
+    of their memory, what lies between them never let in."""
+    from gatx import diff_attention
+    t = make(N, 9 * N, H, d, dv, dtype, device, seed=N + d)
+    graph, want = graph_of(t, N, device), expect(t, N, grads=False)["out"]
+    n = 2 * H * d
+    fused = torch.full((N, n + 3), float("nan"), dtype=dtype, device=device)
+    fused[:, 3:] = t["q"].reshape(N, n)
+    nodes = torch.arange(N - 1, -1, -1, device=device)
+    with torch.no_grad():
+        for q in (t["q"], fused[:, 3:].unflatten(1, (H, 2, d))):
+            ref.check(diff_attention(q, t["k"], t["v"], t["lam"], graph), want, "out")
+            served = diff_attention(q[nodes], t["k"], t["v"], t["lam"], graph, nodes=nodes)
+            ref.check(served, tuple(x[nodes.cpu()] for x in want), "served")
+        q = t["q"][:1].expand(N, H, 2, d)   # one row for all of them
+        same = {**t, "q": q}
+        ref.check(diff_attention(q, t["k"], t["v"], t["lam"], graph),
+                  expect(same, N, grads=False)["out"], "expanded")
