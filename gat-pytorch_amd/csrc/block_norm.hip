@@ -15,6 +15,9 @@
 // lane holds at most 16 elements of each stream (the backward has five of them and two sums). The
 // backward's workgroups walk the rows in a fixed stride and keep A and B in registers; their
 // partial sums are added in workgroup order by a second launch.
+//
+// 44 900 x 1024 bf16, every part there: forward 82 us (460 MB, 5.6 TB/s), backward 192 (736 MB, 3.8
+// TB/s: the loads of a row wait for its two sums), column sums 5.
 #include "dtypes.h"
 
 namespace gatx {

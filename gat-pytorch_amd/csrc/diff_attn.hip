@@ -26,6 +26,12 @@
 // L2, and the sums of pieces (rows of more than hub_edges edges) are plain. A serving call takes
 // one kernel with a running softmax instead: its rows are cut into pieces whose partial results
 // carry their maxima, and it needs no array of logits. Every sum has a fixed order.
+//
+// 44 900 nodes, 1.27 M edges, 4 heads, bf16 d = 128, dv = 256: logits 205 us, values 181, A 163, B 207,
+// C 390 (2.6 GB gathered by each, 5.2 GB by C: 12.6 to 15.9 TB/s, 82 to 89% of it from L2). The
+// gathers of the values pass alone take 170 us, and its vector units never wait either (1.00
+// instructions a cycle and CU; B and C 0.85, the dot products 0.6).
+// One node of 65 537 edges, 8 heads, bf16 d = 64, dv = 128: 48 us and 7 for the join = 5.5 TB/s.
 #include "dtypes.h"
 
 namespace gatx {
@@ -385,8 +391,8 @@ struct Lane {
 };
 // Chunk `at` of map m of a row of q. Unpacked rows (d as it is, any alignment) are read once a row
 // anyway, as whole unaligned chunks whose elements past d are dropped; a chunk that would pass the
-// end of q, element by element. (44 900 x 6 heads of d = 61 in float32: packing 160 -> 100 us, the logits 335 ->
-// 353.)
+// end of q, element by element. (44 900 x 6 heads of d = 61 in float32: packing 160 -> 100 us, the
+// logits 335 -> 353.)
 template <typename T>
 __device__ inline Raw<T> load_q(const AttnArgs& a, int64_t row, int head, int m, int at) {
   if (a.q_end == 0)

@@ -9,6 +9,10 @@
 // first; the row's few taught classes are then written again by the same workgroup, the slots of
 // one class added in slot order, so the result does not depend on the order of anything.
 //
+// 8192 x 32000 bf16, K = 64: forward 149 us (3.5 TB/s; a plain read of the logits 140), backward 200
+// (5.2 TB/s; their copy 205). 44 900 x 121 float32, K = 16: 20 + 22 us (1.5 and 2.4 TB/s, of logits
+// that the L2s and the memory-side cache hold): exp2 and the slots' exchanges.
+//
 // Rows of up to 1024 classes and 64 slots: a group of 8..64 lanes of a wave each, walking the rows
 // in a fixed stride. Wider rows: a workgroup each, 16-byte accesses from the first aligned element
 // on (rows of an odd number of classes start anywhere).
