@@ -65,6 +65,13 @@ __device__ inline Raw<float> load8<float>(const float* p) {
   r.b = *reinterpret_cast<const float4*>(p + 4);
   return r;
 }
+// From any address (global loads need no alignment).
+template <typename T>
+__device__ inline Raw<T> load8_anywhere(const T* p) {
+  Raw<T> r;
+  __builtin_memcpy(&r, p, sizeof(r));
+  return r;
+}
 template <typename T>
 __device__ inline Raw<T> keep8(bool keep, Raw<T> x) {
   x.v.x = keep ? x.v.x : 0u;
@@ -78,6 +85,28 @@ __device__ inline Raw<float> keep8(bool keep, Raw<float> x) {
   x.b = make_float4(keep ? x.b.x : 0.f, keep ? x.b.y : 0.f, keep ? x.b.z : 0.f, keep ? x.b.w : 0.f);
   return x;
 }
+
+// Elements [from, 8) alone.
+template <typename T>
+struct From {
+  uint32_t m[2 * sizeof(T)];
+  __device__ From(int from) {
+#pragma unroll
+    for (int i = 0; i < (int)(2 * sizeof(T)); ++i) {
+      if (sizeof(T) == 4) m[i] = i >= from ? ~0u : 0u;
+      else m[i] = (2 * i >= from ? 0xffffu : 0u) | (2 * i + 1 >= from ? 0xffff0000u : 0u);
+    }
+  }
+  __device__ Raw<T> operator()(const Raw<T>& x) const {
+    uint32_t w[2 * sizeof(T)];
+    __builtin_memcpy(w, &x, sizeof(w));
+#pragma unroll
+    for (int i = 0; i < (int)(2 * sizeof(T)); ++i) w[i] &= m[i];
+    Raw<T> r;
+    __builtin_memcpy(&r, w, sizeof(r));
+    return r;
+  }
+};
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
@@ -350,6 +379,7 @@ struct AttnArgs {
   const void *q, *k, *v, *go;
   int64_t ldq, ldk, ldv, ldgo;
   int64_t q_end;             // elements of an unpacked q; 0: packed
+  int kv_plain;              // serving: k and v as they come too
   int d, dv, dp, dvp;
   const int32_t* col;        // (C: scol)
   const int32_t* seid;       // C
@@ -500,18 +530,29 @@ __device__ inline void serve_step(const Raw<T> (&k1)[U], const Raw<T> (&k2)[U],
   }
 }
 
-// The serving form: one pass with running maxima and sums, each slot its own edges.
+// The serving form: one pass with running maxima and sums, each slot its own edges. Rows of k and v as
+// they come (any alignment, d and dv of 8 or more): packing every node's for a few rows would be most
+// of the call (70 000 nodes, 8 heads of d = 61, dv = 121 in bf16: about 110 us, the call itself 9 us for
+// 30 edges and 61 us for 65 537). The last chunk of a row then starts early enough to end with it; what it shares
+// with the chunk before is left out of q and k, and stored twice alike of the values.
 template <typename T, int G, int NV, bool BIAS>
 __global__ void __launch_bounds__(256) diff_serve_kernel(AttnArgs a) {
   constexpr int U = sizeof(T) == 4 ? 2 : 4;
   const Item it = find_item(a.w);
-  const Lane<G, NV> l(a.w.gs, a.dp, a.dvp);
+  Lane<G, NV> l(a.w.gs, a.dp, a.dvp);
+  const int wd = a.kv_plain ? a.d : a.dp, wv = a.kv_plain ? a.dv : a.dvp;
+  const int chunk = l.at_d;
+  l.at_d = min(l.at_d, wd - 8);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) l.at_dv[i] = min(l.at_dv[i], wv - 8);
+  const From<T> own(chunk - l.at_d);
   const bool has = it.row >= 0;
   const int64_t row = has ? it.row : 0;
-  const Raw<T> q1 = load_q<T>(a, row, it.head, 0, l.at_d), q2 = load_q<T>(a, row, it.head, 1, l.at_d);
+  const Raw<T> q1 = own(load_q<T>(a, row, it.head, 0, l.at_d));
+  const Raw<T> q2 = own(load_q<T>(a, row, it.head, 1, l.at_d));
   Acc<NV> acc;
-  const T* kb = (const T*)a.k + (int64_t)it.head * 2 * a.dp + l.at_d;
-  const T* vb = (const T*)a.v + (int64_t)it.head * a.dvp;
+  const T* kb = (const T*)a.k + (int64_t)it.head * 2 * wd + l.at_d;
+  const T* vb = (const T*)a.v + (int64_t)it.head * wv;
   const int turns = turns_of(wave_max(it.n), l.slots * U);
   for (int t = 0; t < turns; ++t) {
     Raw<T> k1[U], k2[U], v[U][NV];
@@ -528,10 +569,15 @@ __global__ void __launch_bounds__(256) diff_serve_kernel(AttnArgs a) {
         open[u] = open[u] && b[u] != -kInf;
       }
       all = all && open[u];
-      k1[u] = load8(kb + e.j * a.ldk);
-      k2[u] = load8(kb + e.j * a.ldk + a.dp);
+      k1[u] = load8_anywhere(kb + e.j * a.ldk);
+      k2[u] = load8_anywhere(kb + e.j * a.ldk + wd);
 #pragma unroll
-      for (int i = 0; i < NV; ++i) v[u][i] = load8(vb + e.j * a.ldv + l.at_dv[i]);
+      for (int i = 0; i < NV; ++i) v[u][i] = load8_anywhere(vb + e.j * a.ldv + l.at_dv[i]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      k1[u] = own(k1[u]);
+      k2[u] = own(k2[u]);
     }
     if (__all(all))
       serve_step<T, G, NV, U, BIAS, false>(k1, k2, v, q1, q2, b, open, l.in_d, a.scale, acc);
@@ -556,13 +602,18 @@ __global__ void __launch_bounds__(256) diff_serve_kernel(AttnArgs a) {
     slots_sum<G>(acc.a2[j], a.w.gs);
   }
   if (!has || slot != 0) return;
+  // where the chunks go: past the end there is nothing to write but what a plain row's last has
+  int at[NV];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) at[j] = a.kv_plain ? l.at_dv[j] : (c + j * G) * 8;
+  const bool whole = a.dv == a.dvp;
   if (it.slot >= 0) {   // a piece: {m1, l1, m2, l2, sums of map 1, of map 2}
     float* p = a.part + ((int64_t)it.slot * a.w.heads + it.head) * a.part_width;
     if (c == 0) *(float4*)p = make_float4(m1, it.bad ? __builtin_nanf("") : l1, m2, l2);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      store8(p + 4, (c + j * G) * 8, a.dvp, true, acc.a1[j]);
-      store8(p + 4 + a.dvp, (c + j * G) * 8, a.dvp, true, acc.a2[j]);
+      store8(p + 4, at[j], a.dvp, whole, acc.a1[j]);
+      store8(p + 4 + a.dvp, at[j], a.dvp, whole, acc.a2[j]);
     }
     return;
   }
@@ -577,7 +628,7 @@ __global__ void __launch_bounds__(256) diff_serve_kernel(AttnArgs a) {
       o[i] = acc.a1[j][i] * i1 - acc.a2[j][i] * w2;
       if (it.bad) o[i] = __builtin_nanf("");
     }
-    store8(out, (c + j * G) * 8, a.dv, a.dv == a.dvp, o);
+    store8(out, at[j], a.dv, whole, o);
   }
 }
 
@@ -1383,14 +1434,17 @@ extern "C" int gatx_diff_attention(int dtype, const void* q, int64_t ldq, const 
                                    int64_t hub_bound, void* part, size_t part_bytes,
                                    gatx_stream_t s) {
   const bool plain_q = dtype >= 0 && (dtype & GATX_Q_UNPACKED);
-  if (plain_q) dtype &= ~GATX_Q_UNPACKED;
+  const bool plain_kv = dtype >= 0 && (dtype & GATX_KV_UNPACKED);
+  if (dtype >= 0) dtype &= ~(GATX_Q_UNPACKED | GATX_KV_UNPACKED);
   GATX_CALL(check_dims("diff_attention", dtype, heads, d, dv, E, std::max(rows, num_nodes)));
   if (rows == 0) return 0;
   GATX_REQUIRE(q && k && v && rowptr && col && lam && out, "diff_attention: null buffer");
   GATX_REQUIRE(nodes || rows == num_nodes, "diff_attention: a row for every node without nodes");
   GATX_REQUIRE(num_nodes > 0, "diff_attention: no nodes");
-  GATX_REQUIRE((plain_q ? ldq >= 0 : chunked(dtype, q, ldq)) && chunked(dtype, k, ldk) &&
-                   chunked(dtype, v, ldv),
+  GATX_REQUIRE(!plain_kv || (nodes && plain_q && d >= 8 && dv >= 8 && ldk >= 0 && ldv >= 0),
+               "diff_attention: k and v as they come need nodes, q as it comes, d and dv >= 8");
+  GATX_REQUIRE((plain_q ? ldq >= 0 : chunked(dtype, q, ldq)) &&
+                   (plain_kv || (chunked(dtype, k, ldk) && chunked(dtype, v, ldv))),
                "diff_attention: rows of q, k, v must be 16-byte aligned (pack them)");
   GATX_REQUIRE(aligned16(out), "diff_attention: out must be 16-byte aligned");
   GATX_REQUIRE(!bias == !bucket, "diff_attention: bias and bucket go together");
@@ -1399,6 +1453,7 @@ extern "C" int gatx_diff_attention(int dtype, const void* q, int64_t ldq, const 
   AttnArgs a = {};
   a.q = q; a.k = k; a.v = v; a.ldq = ldq; a.ldk = ldk; a.ldv = ldv;
   a.q_end = plain_q ? (rows - 1) * ldq + (int64_t)2 * heads * d : 0;
+  a.kv_plain = plain_kv;
   a.d = d; a.dv = dv; a.dp = (int)round_up(d, 8); a.dvp = (int)round_up(dv, 8);
   a.col = col; a.E = E; a.scale = scale; a.lam = lam; a.bias = bias; a.bucket = bucket;
   a.S = (float2*)S; a.stat = (float4*)stat; a.out = out;

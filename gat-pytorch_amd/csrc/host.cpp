@@ -398,10 +398,17 @@ std::array<Rows, 3> chunked(const Tensor& q, const Tensor& k, const Tensor& v, i
   return out;
 }
 
-// The same where nothing is gathered from q later: its rows stay as they are. *dtype gets the flag.
+// The same where nothing is gathered from q later: its rows stay as they are, and in the serving form
+// those of k and v where they can. *dtype gets the flags.
 std::array<Rows, 3> chunked_keys(const Tensor& q, const Tensor& k, const Tensor& v, int H, int d,
-                                 int dv, int* dtype) {
-  std::array<Rows, 3> out = chunked({}, k, v, H, d, dv);
+                                 int dv, bool serving, int* dtype) {
+  std::array<Rows, 3> out;
+  if (serving && d >= 8 && dv >= 8) {
+    out = {Rows(), heads_of(k), heads_of(v)};
+    *dtype |= GATX_KV_UNPACKED;
+  } else {
+    out = chunked({}, k, v, H, d, dv);
+  }
   out[0] = heads_of(q);
   *dtype |= GATX_Q_UNPACKED;
   return out;
@@ -518,7 +525,7 @@ Tensor diff_attention(const Tensor& q, const Tensor& k, const Tensor& v, const T
     if (bias.defined())
       bucket = relative_buckets(csr, *positions_, exact, bounds, bidirectional, {});
     int dtype = code(q.scalar_type());
-    rows = grad ? chunked(q, k, v, H, d, dv) : chunked_keys(q, k, v, H, d, dv, &dtype);
+    rows = grad ? chunked(q, k, v, H, d, dv) : chunked_keys(q, k, v, H, d, dv, false, &dtype);
     out = at::empty({num_nodes, H, dv}, q.options());
     S = floats(q, {H, std::max<int64_t>(edges, 1), 2});
     stat = floats(q, {H, num_nodes, 4});
@@ -574,7 +581,7 @@ Tensor diff_attention_nodes(const Tensor& q, const Tensor& k, const Tensor& v, c
   if (bias.defined())
     bucket = relative_buckets(csr, *positions_, exact, bounds, bidirectional, nodes);
   int dtype = code(q.scalar_type());
-  const auto rows = chunked_keys(q, k, v, H, d, dv, &dtype);
+  const auto rows = chunked_keys(q, k, v, H, d, dv, true, &dtype);
   const Tensor out = at::empty({M, H, dv}, q.options());
   const size_t pb = gatx_diff_attention_part_bytes(pieces > 1 ? M * pieces : 0, H, (dv + 7) / 8 * 8);
   const Tensor part = bytes(q, pb);

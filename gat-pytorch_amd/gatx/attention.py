@@ -180,7 +180,8 @@ def diff_attention(q, k, v, lam, graph: Graph, *, scale=None, bias=None, positio
     """Differential attention of every node over its in-neighbours in `graph`.
 
     q, k: (N, H, 2, d) (both maps' queries and keys), v: (N, H, dv), one dtype; slices of a fused
-    projection are read in place where their rows are 16-byte aligned and d, dv multiples of 8.
+    projection are read in place where their rows are 16-byte aligned and d, dv multiples of 8, and
+    packed in one launch otherwise (with nodes: read as they are, but for widths below 8).
     lam: (H,). scale: 1 / sqrt(d) unless given. Returns (N, H, dv). A node without in-edges (or with
     every one of them shut) gets zeros.
 

@@ -642,7 +642,8 @@ int gatx_diff_attention_pack(int dtype, int64_t rows, int64_t keys, int num_head
  * them of scale q[i,h,m] . k[col[e],h,m] + bias[bucket[e],h] (bias NULL: none; an entry of -inf
  * shuts its bucket, whatever lies in the keys and values behind it). q: rows x (H,2,dp), k: keys x
  * (H,2,dp), v: keys x (H,dvp), chunked as above (zero tails), row strides ld*; with GATX_Q_UNPACKED
- * or'ed to dtype q is rows x (H,2,d) as it comes (ldq >= 0; the backward takes chunked rows only);
+ * or'ed to dtype q is rows x (H,2,d) as it comes (ldq >= 0; the backward takes chunked rows only),
+ * and with GATX_KV_UNPACKED (nodes, GATX_Q_UNPACKED, d >= 8 and dv >= 8 only) so are k and v;
  * out: rows x (H,dv), packed, of `dtype`. A row without open edges gives zeros. d <= 256, dv <= 512.
  * col (and bucket, and below seid) have at least one readable entry, E = 0 or not.
  * nodes (nullable): q row r is node nodes[r]'s (its CSR row; keys = num_nodes), each row's edges
@@ -652,6 +653,7 @@ int gatx_diff_attention_pack(int dtype, int64_t rows, int64_t keys, int num_head
  * Without nodes S (H x max(E, 1) x 2 logits) and stat (H x rows x {max1, 1/sum1, max2, 1/sum2}) are
  * written, for the backward. part: gatx_diff_attention_part_bytes(rows * pieces, or hub_bound). */
 #define GATX_Q_UNPACKED 16
+#define GATX_KV_UNPACKED 32
 size_t gatx_diff_attention_part_bytes(int64_t slots, int num_heads, int dvp);
 int gatx_diff_attention(int dtype, const void* q, int64_t ldq, const void* k, int64_t ldk,
                         const void* v, int64_t ldv, int num_heads, int d, int dv,

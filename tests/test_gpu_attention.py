@@ -396,3 +396,27 @@ def test_queries_read_where_they_are(H, d, dv, N, dtype, device):
         same = {**t, "q": q}
         ref.check(diff_attention(q, t["k"], t["v"], t["lam"], graph),
                   expect(same, N, grads=False)["out"], "expanded")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H,d,dv", [(1, 8, 8), (2, 9, 15), (3, 61, 121), (1, 250, 509), (2, 16, 17),
+                                    (4, 17, 16), (2, 7, 12), (2, 12, 7)])
+@pytest.mark.parametrize("hub", [0, 3000])
+def test_serving_reads_keys_and_values_where_they_are(H, d, dv, hub, dtype, device):
+    """Any width and alignment, NaN between the rows; one piece a row and many."""
+    from gatx import diff_attention
+    N = 50
+    t = make(N, 300, H, d, dv, dtype, device, seed=d + hub, hub=hub)
+    graph = graph_of(t, N, device)
+    nodes = torch.tensor([0, N - 1, 7, 7, 1], device=device)
+    want = expect(t, N, grads=False)["out"]
+    want = tuple(x[nodes.cpu()] for x in want)
+    nk, nv = 2 * H * d, H * dv
+    fused = torch.full((N, 1 + nk + 1 + nv), float("nan"), dtype=dtype, device=device)
+    fused[:, 1:1 + nk] = t["k"].reshape(N, nk)
+    fused[:, 2 + nk:] = t["v"].reshape(N, nv)
+    k, v = fused[:, 1:1 + nk].unflatten(1, (H, 2, d)), fused[:, 2 + nk:].unflatten(1, (H, dv))
+    with torch.no_grad():
+        for kk, vv in ((t["k"], t["v"]), (k, v)):
+            got = diff_attention(t["q"][nodes], kk, vv, t["lam"], graph, nodes=nodes)
+            ref.check(got, want, "served")
