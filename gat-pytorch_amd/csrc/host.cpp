@@ -419,16 +419,17 @@ struct Csr {
   Tensor rowptr, col, rowidx;
   int64_t num_nodes = 0, edges = 0;   // edges: the allocation's bound
 };
-// A plan of long rows' pieces: (edges a piece, entries, their number, the plan's bound).
-using Plan = std::tuple<int64_t, Opt, Opt, int64_t>;
+// A plan of long rows' pieces: (edges a piece, entries, their number, the plan's bound), and the rows by
+// length (none: as they are).
+using Plan = std::tuple<int64_t, Opt, Opt, int64_t, Opt>;
 struct Hubs {
   int edges = 0;
-  Tensor hubs, count;
+  Tensor hubs, count, order;
   int64_t bound = 0;
   Hubs() = default;
   explicit Hubs(const Plan& p)
       : edges((int)std::get<0>(p)), hubs(of(std::get<1>(p))), count(of(std::get<2>(p))),
-        bound(std::get<3>(p)) {}
+        order(of(std::get<4>(p))), bound(std::get<3>(p)) {}
 };
 const int32_t* ints(const Tensor& t) { return (const int32_t*)ptr(t); }
 
@@ -445,7 +446,8 @@ struct DiffAttentionBackward : public Node {
     for (auto* s : {&q, &k, &v, &lam, &bias}) s->reset_data();
     for (auto& r : copies) r.t.reset();
     for (auto* t : {&bucket, &S, &stat, &srowptr, &scol, &seid, &csr.rowptr, &csr.col, &csr.rowidx,
-                    &hubs.hubs, &hubs.count, &src_hubs.hubs, &src_hubs.count})
+                    &hubs.hubs, &hubs.count, &hubs.order, &src_hubs.hubs, &src_hubs.count,
+                    &src_hubs.order})
       t->reset();
   }
   variable_list apply(variable_list&& go) override {
@@ -484,7 +486,7 @@ struct DiffAttentionBackward : public Node {
               fptr(lp), (const uint8_t*)ptr(bucket), nb, fptr(S), fptr(stat), ptr(out[0]),
               ptr(out[1]), ptr(out[2]), fptr(out[3]), fptr(out[4]), hubs.edges, ints(hubs.hubs),
               ints(hubs.count), hubs.bound, ints(src_hubs.hubs), ints(src_hubs.count), sb, ptr(ws),
-              wb, stream_of(qt)),
+              wb, ints(hubs.order), ints(src_hubs.order), stream_of(qt)),
           "diff_attention_backward");
     }
     return once(std::move(out), "diff_attention");
@@ -536,7 +538,7 @@ Tensor diff_attention(const Tensor& q, const Tensor& k, const Tensor& v, const T
                             ints(col), edges, num_nodes, num_nodes, nullptr, 1, (float)scale,
                             fptr(lp), fptr(bp), (const uint8_t*)ptr(bucket), ptr(out), fptr(S),
                             fptr(stat), hubs.edges, ints(hubs.hubs), ints(hubs.count), hubs.bound,
-                            ptr(part), pb, stream_of(q)),
+                            ptr(part), pb, ints(hubs.order), stream_of(q)),
         "diff_attention");
   }
   if (grad) {
@@ -589,7 +591,8 @@ Tensor diff_attention_nodes(const Tensor& q, const Tensor& k, const Tensor& v, c
                           rows[1].ld, ptr(rows[2].t), rows[2].ld, H, d, dv, ints(rowptr), ints(col),
                           edges, M, num_nodes, (const int64_t*)ptr(nodes), (int)pieces,
                           (float)scale, fptr(lam), fptr(bias), (const uint8_t*)ptr(bucket), ptr(out),
-                          nullptr, nullptr, 0, nullptr, nullptr, 0, ptr(part), pb, stream_of(q)),
+                          nullptr, nullptr, 0, nullptr, nullptr, 0, ptr(part), pb, nullptr,
+                          stream_of(q)),
       "diff_attention");
   return out;
 }

@@ -147,13 +147,14 @@ SIGNATURES = {
     "gatx_diff_attention_part_bytes": (c_sz, [c_i64, c_i, c_i]),
     "gatx_diff_attention": (c_i, [c_i, P, c_i64, P, c_i64, P, c_i64, c_i, c_i, c_i, P, P, c_i64,
                                   c_i64, c_i64, P, c_i, c_f, P, P, P, P, P, P, c_i, P, P, c_i64,
-                                  P, c_sz, P]),
+                                  P, c_sz, P, P]),
+    "gatx_diff_attention_row_order": (c_i, [P, c_i64, P, P]),
     "gatx_diff_attention_backward_workspace_bytes": (c_sz, [c_i64, c_i64, c_i, c_i, c_i, c_i,
                                                             c_i64, c_i64]),
     "gatx_diff_attention_backward": (c_i, [c_i, P, c_i64, P, c_i64, P, c_i64, P, c_i64, c_i, c_i,
                                            c_i, P, P, P, P, P, c_i64, c_i64, c_f, P, P, c_i, P, P,
                                            P, P, P, P, P, c_i, P, P, c_i64, P, P, c_i64, P, c_sz,
-                                           P]),
+                                           P, P, P]),
     "gatx_block_norm": (c_i, [c_i, c_i64, c_i64, P, c_i64, P, P, c_i64, P, c_i, c_i64, P, P, c_f,
                               P, P, P, P, P]),
     "gatx_block_norm_backward_workspace_bytes": (c_sz, [c_i64, c_i64]),

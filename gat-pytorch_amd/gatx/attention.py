@@ -16,7 +16,7 @@ import torch
 from torch import nn
 
 from . import tuning
-from ._lib import DTYPES, host as _host, on_device, stream
+from ._lib import DTYPES, call, host as _host, on_device, ptr, stream
 from .graph import Graph, graph_cache
 
 MAX_HEAD_WIDTH = 256    # d
@@ -100,7 +100,34 @@ def _transpose(graph: Graph):
     return graph.srowptr, graph.scol, graph.seid
 
 
+# rows x heads from which rows share a wave
+_ORDER_ITEMS = 8192
+
+
+def _row_order(graph: Graph, heads: int, source: bool):
+    """The rows by length (csrc/diff_attn.hip, row_order_kernel), for rows that share waves. No result
+    depends on it, so a capture that finds none goes without."""
+    if graph.num_nodes * heads < _ORDER_ITEMS:
+        return None
+    key = ("order", source)
+    order = graph._hub_plans.get(key)
+    missing = order is None
+    if missing:
+        if graph._event is not None and torch.cuda.is_current_stream_capturing():
+            return None
+        order = torch.empty((graph.num_nodes, 4), dtype=torch.int32, device=graph.device)
+        call("gatx_diff_attention_row_order", ptr(graph.srowptr if source else graph.rowptr),
+             graph.num_nodes, ptr(order), stream())
+        graph._hub_plans[key] = order
+    _ready(graph, key, missing)
+    return order
+
+
 _NO_PLAN = (0, None, None, 0)
+
+
+def _plan(graph: Graph, heads: int, source: bool):
+    return _hub_plan(graph, source) + (_row_order(graph, heads, source),)
 
 
 def _hub_plan(graph: Graph, source: bool):
@@ -212,11 +239,11 @@ def diff_attention(q, k, v, lam, graph: Graph, *, scale=None, bias=None, positio
         pieces = max(1, min(_SERVING_WAVES // items, 256, -(-graph.edge_bound // 256)))
         return _host.diff_attention_nodes(*args, nodes, pieces)
     with on_device(graph.device):   # (the graph's own launches)
-        transpose, src_plan = (None, None, None), _NO_PLAN
+        transpose, src_plan = (None, None, None), _NO_PLAN + (None,)
         if grad and (k.requires_grad or v.requires_grad):
             transpose = _transpose(graph)
-            src_plan = _hub_plan(graph, True)
-        return _host.diff_attention(*args, _hub_plan(graph, False), *transpose, src_plan)
+            src_plan = _plan(graph, q.size(1), True)
+        return _host.diff_attention(*args, _plan(graph, q.size(1), False), *transpose, src_plan)
 
 
 class DiffAttention(nn.Module):

@@ -651,7 +651,11 @@ int gatx_diff_attention_pack(int dtype, int64_t rows, int64_t keys, int num_head
  * nodes == NULL: rows == num_nodes; rows of more than hub_edges edges run in pieces (a plan of
  * gatx_graph_hub_plan at hub_edges; hub_edges = 0: never).
  * Without nodes S (H x max(E, 1) x 2 logits) and stat (H x rows x {max1, 1/sum1, max2, 1/sum2}) are
- * written, for the backward. part: gatx_diff_attention_part_bytes(rows * pieces, or hub_bound). */
+ * written, for the backward. part: gatx_diff_attention_part_bytes(rows * pieces, or hub_bound).
+ * order (nullable, 16-byte aligned): gatx_diff_attention_row_order's 4 int32 a row of this CSR; it
+ * changes the time, never a result. */
+int gatx_diff_attention_row_order(const int32_t* rowptr, int64_t rows, int32_t* order,
+                                  gatx_stream_t stream);
 #define GATX_Q_UNPACKED 16
 #define GATX_KV_UNPACKED 32
 size_t gatx_diff_attention_part_bytes(int64_t slots, int num_heads, int dvp);
@@ -662,10 +666,11 @@ int gatx_diff_attention(int dtype, const void* q, int64_t ldq, const void* k, in
                         const float* lam, const float* bias, const uint8_t* bucket, void* out,
                         float* S, float* stat, int hub_edges, const int32_t* hubs,
                         const int32_t* hub_count, int64_t hub_bound, void* part,
-                        size_t part_bytes, gatx_stream_t stream);
+                        size_t part_bytes, const int32_t* order, gatx_stream_t stream);
 /* Its gradients from go (num_nodes x (H,dvp), as v): gq, gk (num_nodes x (H,2,d)), gv
  * (num_nodes x (H,dv)), glam (H), gbias (n_buckets x H); each nullable. S and stat are the
- * forward's; srowptr / scol / seid the transposed CSR, with its own hub plan. Fixed-order sums.
+ * forward's; srowptr / scol / seid the transposed CSR, with its own hub plan and order. Fixed-order
+ * sums.
  * workspace: gatx_diff_attention_backward_workspace_bytes(). */
 size_t gatx_diff_attention_backward_workspace_bytes(int64_t num_nodes, int64_t E, int num_heads,
                                                     int d, int dv, int n_buckets,
@@ -681,6 +686,7 @@ int gatx_diff_attention_backward(int dtype, const void* q, int64_t ldq, const vo
                                  const int32_t* hub_count, int64_t hub_bound,
                                  const int32_t* src_hubs, const int32_t* src_hub_count,
                                  int64_t src_hub_bound, void* workspace, size_t workspace_bytes,
+                                 const int32_t* order, const int32_t* src_order,
                                  gatx_stream_t stream);
 
 /* The norms around a block, rows x cols (cols <= 8192), one pass: with rms(z) = z / sqrt(mean z^2 +

@@ -209,7 +209,7 @@ def test_distill_c_refusals():
 def test_attention_c_refusals():
     #      dt q    ldq k    ldk v    ldv H  d  dv rowptr col E  M  N  nodes pieces
     ok = [0, ANY, 32, ANY, 32, ANY, 16, 2, 8, 8, ANY, ANY, 9, 6, 6, None, 1, 1.0, ANY, None, None,
-          ANY, ANY, ANY, 0, None, None, 0, None, 0, None]
+          ANY, ANY, ANY, 0, None, None, 0, None, 0, None, None]
     for at, value in ((0, 4), (1, None), (2, 31), (1, ANY + 4), (4, 31), (7, 0), (8, 257), (9, 513),
                       (12, 1 << 31), (13, 5), (15, ANY), (16, 5000), (19, ANY), (20, ANY),
                       (21, None), (21, ANY + 8), (22, None), (24, 4)):
@@ -228,13 +228,27 @@ def test_attention_c_refusals():
 def test_attention_backward_c_refusals():
     ok = [0, ANY, 32, ANY, 32, ANY, 16, ANY, 16, 2, 8, 8, ANY, ANY, ANY, ANY, ANY, 9, 6, 1.0, ANY,
           None, 0, ANY, ANY, ANY, ANY, ANY, ANY, None, 0, None, None, 0, None, None, 0, ANY,
-          10 ** 9, None]
+          10 ** 9, None, None, None]
     for at, value in ((0, 4), (7, None), (8, 15), (14, None), (22, 257), (29, ANY), (23, None),
                       (25, ANY + 4), (30, 4), (38, 8)):
         bad = list(ok)
         bad[at] = value
         rc, msg = c_call("gatx_diff_attention_backward", *bad)
         assert rc == 1000 and "diff_attention_backward" in msg, (at, msg)
+
+
+def test_row_order_c_refusals():
+    for bad in ((None, 5, ANY, None), (ANY, 5, None, None), (ANY, 5, ANY + 4, None),
+                (ANY, 1 << 31, ANY, None), (ANY, -1, ANY, None)):
+        rc, msg = c_call("gatx_diff_attention_row_order", *bad)
+        assert rc == 1000 and "row_order" in msg, bad
+
+
+def test_order_c_refusals():
+    ok = [0, ANY, 32, ANY, 32, ANY, 16, 2, 8, 8, ANY, ANY, 9, 6, 6, None, 1, 1.0, ANY, None, None,
+          ANY, ANY, ANY, 0, None, None, 0, None, 0, ANY + 4, None]
+    rc, msg = c_call("gatx_diff_attention", *ok)
+    assert rc == 1000 and "order" in msg
 
 
 def test_buckets_c_refusals():

@@ -420,3 +420,35 @@ def test_serving_reads_keys_and_values_where_they_are(H, d, dv, hub, dtype, devi
         for kk, vv in ((t["k"], t["v"]), (k, v)):
             got = diff_attention(t["q"][nodes], kk, vv, t["lam"], graph, nodes=nodes)
             ref.check(got, want, "served")
+
+
+@pytest.mark.parametrize("N,E", [(1, 0), (2047, 9000), (2048, 0), (2049, 60000), (6000, 40000)])
+def test_rows_by_length(N, E, device):
+    """A stable sort of every 2048 rows by pairs of edges (1022 and more alike), longest first."""
+    from gatx._lib import call, ptr, stream
+    t = make(N, E, 1, 8, 8, torch.float32, device, seed=N, hub=1500 if N == 6000 else 0)
+    graph = graph_of(t, N, device)
+    order = torch.full((N, 4), -1, dtype=torch.int32, device=device)
+    call("gatx_diff_attention_row_order", ptr(graph.rowptr), N, ptr(order), stream())
+    rowptr = graph.rowptr.cpu().long()
+    length = rowptr[1:] - rowptr[:-1]
+    key = ((length + 1) // 2).clamp(max=511)
+    rows = torch.cat([c[torch.sort(key[c], descending=True, stable=True).indices]
+                      for c in torch.arange(N).split(2048)])
+    assert torch.equal(order.cpu().long(), torch.stack(
+        [rows, rowptr[:-1][rows], length[rows], torch.zeros(N, dtype=torch.int64)], 1))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d,dv", [(16, 24), (8, 300)])
+def test_row_order_changes_no_bit(d, dv, dtype, device, monkeypatch):
+    from gatx import attention
+    N, H = 3000, 6
+    t = make(N, 30000, H, d, dv, dtype, device, seed=8, hub=2000, buckets=8)
+    assert N * H >= attention._ORDER_ITEMS
+    a = run(t, graph_of(t, N, device))
+    monkeypatch.setattr(attention, "_ORDER_ITEMS", 1 << 40)
+    b = run(t, graph_of(t, N, device))
+    check_all(a, expect(t, N))
+    for n in a:
+        assert torch.equal(a[n], b[n]), n
