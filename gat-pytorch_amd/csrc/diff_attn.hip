@@ -160,6 +160,31 @@ __device__ inline void unpack8(const Raw<float>& x, float (&f)[8]) {
   f[0] = x.a.x; f[1] = x.a.y; f[2] = x.a.z; f[3] = x.a.w;
   f[4] = x.b.x; f[5] = x.b.y; f[6] = x.b.z; f[7] = x.b.w;
 }
+// Whether an edge's row counts, as unpacking uses it: bf16 pairs are unpacked by one instruction an
+// element that can also clear it (the mask of the upper half, the byte selector of the lower).
+template <typename T>
+struct Keep {
+  int keep;
+  __device__ Keep(bool open) : keep(open) {}
+  template <int G, int I>
+  __device__ Keep of_edge() const;
+  __device__ void unpack(const Raw<T>& x, float (&f)[8]) const { unpack8(keep8(keep != 0, x), f); }
+};
+template <>
+struct Keep<__bf16> {
+  int hi, sel;
+  __device__ Keep(bool open) : hi(open ? (int)0xffff0000u : 0), sel(open ? 0x01000c0c : 0x0c0c0c0c) {}
+  template <int G, int I>
+  __device__ Keep of_edge() const;
+  __device__ void unpack(const Raw<__bf16>& x, float (&f)[8]) const {
+    const uint32_t w[4] = {x.v.x, x.v.y, x.v.z, x.v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[2 * i] = __uint_as_float(__builtin_amdgcn_perm(w[i], w[i], (uint32_t)sel));
+      f[2 * i + 1] = __uint_as_float(w[i] & (uint32_t)hi);
+    }
+  }
+};
 __device__ inline void axpy8(float p, const float (&x)[8], float (&acc)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) acc[i] = fmaf(p, x[i], acc[i]);
@@ -267,6 +292,37 @@ template <int G, int I>
 __device__ inline int64_t tile_get(int64_t x) {
   const uint32_t lo = (uint32_t)tile_get<G, I>((int)x);
   return ((int64_t)tile_get<G, I>((int)(x >> 32)) << 32) | lo;
+}
+template <typename T>
+template <int G, int I>
+__device__ inline Keep<T> Keep<T>::of_edge() const {
+  Keep k = *this;
+  k.keep = tile_get<G, I>(keep);
+  return k;
+}
+template <int G, int I>
+__device__ inline Keep<__bf16> Keep<__bf16>::of_edge() const {
+  Keep k = *this;
+  k.hi = tile_get<G, I>(hi);
+  k.sel = tile_get<G, I>(sel);
+  return k;
+}
+template <bool ALL, typename T>
+__device__ inline void axpy_kept(float p, const Raw<T>& x, const Keep<T>& k, float (&acc)[8]) {
+  float f[8];
+  if (ALL) unpack8(x, f);
+  else k.unpack(x, f);
+  axpy8(p, f, acc);
+}
+// A gathered row's offset and where it is: in bytes for the 16-bit types (an instruction less a load),
+// in elements for float32 (PPI, d = 61: logits 353 us, 365 in bytes).
+template <typename T>
+__device__ inline int64_t row_off(int64_t j, int64_t ld) {
+  return j * ld * (sizeof(T) == 2 ? 2 : 1);
+}
+template <typename T>
+__device__ inline const T* row_at(const T* p, int64_t off) {
+  return sizeof(T) == 2 ? (const T*)((const char*)p + off) : p + off;
 }
 // Sums of a tile's values over the G lanes of an edge: the lane that holds edge i gets v[i]'s.
 template <int G>
@@ -802,7 +858,7 @@ __global__ void __launch_bounds__(256) diff_score_kernel(AttnArgs a) {
   for (int t = 0; !tl.done(t, 0); ++t) {
     const int o = tl.first(t, l.slot) + tl.mine;
     const Edge e(it, o, a.col);
-    const int64_t off = e.j * a.ldk;
+    const int64_t off = row_off<T>(e.j, a.ldk);
     float b = 0.f;
     if (BIAS) {
       const int bk = a.bucket[e.e];   // (past the end: not necessarily one)
@@ -819,7 +875,7 @@ __global__ void __launch_bounds__(256) diff_score_kernel(AttnArgs a) {
       Raw<T> k1[U], k2[U];
       each<U>([&](auto I) {
         constexpr int u = decltype(I)::value;
-        const T* p = kb + tile_get<G, b0 + u>(off);
+        const T* p = row_at(kb, tile_get<G, b0 + u>(off));
         k1[u] = load8(p);
         k2[u] = load8(p + a.dp);
       });
@@ -874,9 +930,10 @@ __global__ void __launch_bounds__(256) diff_value_kernel(AttnArgs a) {
   float acc[NV][8] = {};
   for (int t = 0; !tl.done(t, 0); ++t) {
     const Edge e(it, tl.first(t, l.slot) + tl.mine, a.col);
-    const int64_t off = e.j * a.ldv;
+    const int64_t off = row_off<T>(e.j, a.ldv);
     const float2 x = a.S[he + e.e], p = weights(x, st);
-    const int open = e.in && (x.x != -kInf || x.y != -kInf);
+    const bool open = e.in && (x.x != -kInf || x.y != -kInf);
+    const Keep<T> keep(open);
     const float w = open ? p.x - lam * p.y : 0.f;
     auto edges = [&](auto ALL) {
       each<NL / U>([&](auto B) {
@@ -885,17 +942,16 @@ __global__ void __launch_bounds__(256) diff_value_kernel(AttnArgs a) {
         Raw<T> v[U][NV];
         each<U>([&](auto I) {
           constexpr int u = decltype(I)::value;
-          const T* p = vb + tile_get<G, b0 + u>(off);
+          const T* p = row_at(vb, tile_get<G, b0 + u>(off));
 #pragma unroll
           for (int i = 0; i < NV; ++i) v[u][i] = load8(p + l.at_dv[i]);
         });
         each<U>([&](auto I) {
           constexpr int u = decltype(I)::value;
           const float wu = tile_get<G, b0 + u>(w);
-          const bool keep = decltype(ALL)::value || tile_get<G, b0 + u>(open);
+          const Keep<T> ku = keep.template of_edge<G, b0 + u>();
 #pragma unroll
-          for (int i = 0; i < NV; ++i)
-            axpy8(wu, decltype(ALL)::value ? v[u][i] : keep8(keep, v[u][i]), acc[i]);
+          for (int i = 0; i < NV; ++i) axpy_kept<decltype(ALL)::value>(wu, v[u][i], ku, acc[i]);
         });
       });
     };
@@ -987,7 +1043,7 @@ __global__ void __launch_bounds__(256) diff_dw_kernel(AttnArgs a) {
   float d[2] = {0.f, 0.f};
   for (int t = 0; !tl.done(t, 0); ++t) {
     const Edge e(it, tl.first(t, l.slot) + tl.mine, a.col);
-    const int64_t off = e.j * a.ldv;
+    const int64_t off = row_off<T>(e.j, a.ldv);
     const float2 x = a.S[he + e.e];
     float y[NL];
     each<NL / U>([&](auto B) {
@@ -1000,7 +1056,7 @@ __global__ void __launch_bounds__(256) diff_dw_kernel(AttnArgs a) {
       Raw<T> v[U][NV];
       each<U>([&](auto I) {
         constexpr int u = decltype(I)::value;
-        const T* p = vb + tile_get<G, b0 + u>(off);
+        const T* p = row_at(vb, tile_get<G, b0 + u>(off));
 #pragma unroll
         for (int i = 0; i < NV; ++i) v[u][i] = load8(p + l.at_dv[i]);
       });
@@ -1057,15 +1113,16 @@ __global__ void __launch_bounds__(256) diff_gq_kernel(AttnArgs a) {
   const float4 st = a.stat[sr];
   const float2 D = a.D[sr];
   const float lam = a.lam[it.head];
-  const T* kb = (const T*)a.k + (int64_t)it.head * 2 * a.dp + l.at_d;
+  const T* kb = (const T*)a.k + (int64_t)it.head * 2 * a.dp + l.at_d, *kb2 = kb + a.dp;
   const int64_t he = (int64_t)it.head * a.E;
   float g1[8] = {}, g2[8] = {};
   for (int t = 0; !tl.done(t, 0); ++t) {
     const Edge e(it, tl.first(t, l.slot) + tl.mine, a.col);
-    const int64_t off = e.j * a.ldk;
+    const int64_t off = row_off<T>(e.j, a.ldk);
     const float2 x = a.S[he + e.e], p = weights(x, st);
     const float dw = a.dw[he + e.e];
-    const int open = e.in && (x.x != -kInf || x.y != -kInf);
+    const bool open = e.in && (x.x != -kInf || x.y != -kInf);
+    const Keep<T> keep(open);
     const float x1 = open ? p.x * (dw - D.x) : 0.f;
     const float x2 = open ? -lam * p.y * (dw - D.y) : 0.f;
     if (e.in && tl.owner)
@@ -1079,16 +1136,16 @@ __global__ void __launch_bounds__(256) diff_gq_kernel(AttnArgs a) {
         Raw<T> k1[U], k2[U];
         each<U>([&](auto I) {
           constexpr int u = decltype(I)::value;
-          const T* p = kb + tile_get<G, b0 + u>(off);
-          k1[u] = load8(p);
-          k2[u] = load8(p + a.dp);
+          const int64_t at = tile_get<G, b0 + u>(off);
+          k1[u] = load8(row_at(kb, at));
+          k2[u] = load8(row_at(kb2, at));
         });
         each<U>([&](auto I) {
           constexpr int u = decltype(I)::value;
           const float y1 = tile_get<G, b0 + u>(x1), y2 = tile_get<G, b0 + u>(x2);
-          const bool keep = decltype(ALL)::value || tile_get<G, b0 + u>(open);
-          axpy8(y1, decltype(ALL)::value ? k1[u] : keep8(keep, k1[u]), g1);
-          axpy8(y2, decltype(ALL)::value ? k2[u] : keep8(keep, k2[u]), g2);
+          const Keep<T> ku = keep.template of_edge<G, b0 + u>();
+          axpy_kept<decltype(ALL)::value>(y1, k1[u], ku, g1);
+          axpy_kept<decltype(ALL)::value>(y2, k2[u], ku, g2);
         });
       });
     };
@@ -1123,17 +1180,20 @@ __global__ void __launch_bounds__(256) diff_gkv_kernel(AttnArgs a) {
   const Tiles<G> tl(it, a.w.gs);
   const bool has = it.row >= 0;
   const int64_t row = has ? it.row : 0;
-  const T* qb = (const T*)a.q + (int64_t)it.head * 2 * a.dp + l.at_d;
-  const T* gb = (const T*)a.go + (int64_t)it.head * a.dvp;
+  const T* qb = (const T*)a.q + (int64_t)it.head * 2 * a.dp + l.at_d, *qb2 = qb + a.dp;
+  const T* gb[NV];
+#pragma unroll
+  for (int k = 0; k < NV; ++k) gb[k] = (const T*)a.go + (int64_t)it.head * a.dvp + l.at_dv[k];
   const float4* rec = a.rec + (int64_t)it.head * a.E;
   float g1[8] = {}, g2[8] = {}, gv[NV][8] = {};
   for (int t = 0; !tl.done(t, 0); ++t) {
     const Edge e(it, tl.first(t, l.slot) + tl.mine, a.col);
-    const int64_t offq = e.j * a.ldq, offg = e.j * a.ldgo;
+    const int64_t offq = row_off<T>(e.j, a.ldq), offg = row_off<T>(e.j, a.ldgo);
     const int id = a.seid[e.e];
     const float4 r = rec[it.n > 0 ? id : 0];
     // a shut edge is all zeros: what it points at does not count
-    const int open = e.in && (r.x != 0.f || r.y != 0.f || r.z != 0.f);
+    const bool open = e.in && (r.x != 0.f || r.y != 0.f || r.z != 0.f);
+    const Keep<T> keep(open);
     const float r1 = open ? r.x : 0.f, r2 = open ? r.y : 0.f, rw = open ? r.z : 0.f;
     auto edges = [&](auto ALL) {
       each<NL / U>([&](auto B) {
@@ -1142,23 +1202,22 @@ __global__ void __launch_bounds__(256) diff_gkv_kernel(AttnArgs a) {
         Raw<T> q1[U], q2[U], go[U][NV];
         each<U>([&](auto I) {
           constexpr int u = decltype(I)::value;
-          const T* p = qb + tile_get<G, b0 + u>(offq);
-          q1[u] = load8(p);
-          q2[u] = load8(p + a.dp);
-          const T* g = gb + tile_get<G, b0 + u>(offg);
+          const int64_t at = tile_get<G, b0 + u>(offq), atg = tile_get<G, b0 + u>(offg);
+          q1[u] = load8(row_at(qb, at));
+          q2[u] = load8(row_at(qb2, at));
 #pragma unroll
-          for (int k = 0; k < NV; ++k) go[u][k] = load8(g + l.at_dv[k]);
+          for (int k = 0; k < NV; ++k) go[u][k] = load8(row_at(gb[k], atg));
         });
         each<U>([&](auto I) {
           constexpr int u = decltype(I)::value;
           constexpr bool all = decltype(ALL)::value;
-          const bool keep = all || tile_get<G, b0 + u>(open);
+          const Keep<T> ku = keep.template of_edge<G, b0 + u>();
           const float w1 = tile_get<G, b0 + u>(r1), w2 = tile_get<G, b0 + u>(r2),
                       w = tile_get<G, b0 + u>(rw);
-          axpy8(w1, all ? q1[u] : keep8(keep, q1[u]), g1);
-          axpy8(w2, all ? q2[u] : keep8(keep, q2[u]), g2);
+          axpy_kept<all>(w1, q1[u], ku, g1);
+          axpy_kept<all>(w2, q2[u], ku, g2);
 #pragma unroll
-          for (int k = 0; k < NV; ++k) axpy8(w, all ? go[u][k] : keep8(keep, go[u][k]), gv[k]);
+          for (int k = 0; k < NV; ++k) axpy_kept<all>(w, go[u][k], ku, gv[k]);
         });
       });
     };
