@@ -27,10 +27,10 @@
 // one kernel with a running softmax instead: its rows are cut into pieces whose partial results
 // carry their maxima, and it needs no array of logits. Every sum has a fixed order.
 //
-// 44 900 nodes, 1.27 M edges, 4 heads, bf16 d = 128, dv = 256: logits 205 us, values 181, A 163, B 207,
-// C 390 (2.6 GB gathered by each, 5.2 GB by C: 12.6 to 15.9 TB/s, 82 to 89% of it from L2). The
-// gathers of the values pass alone take 170 us, and its vector units never wait either (1.00
-// instructions a cycle and CU; B and C 0.85, the dot products 0.6).
+// 44 900 nodes, 1.27 M edges, 4 heads, bf16 d = 128, dv = 256: logits 198 us, values 168, A 160, B
+// 190, C 370 (2.6 GB gathered by each, 5.2 GB by C: 13 to 16 TB/s, 74 to 87% of it from L2). The
+// vector units issue 0.85 instructions a cycle and CU in the values pass, 0.7 in B and C, 0.55 in
+// the dot products.
 // One node of 65 537 edges, 8 heads, bf16 d = 64, dv = 128: 48 us and 7 for the join = 5.5 TB/s.
 #include "dtypes.h"
 
@@ -664,11 +664,12 @@ __device__ inline void serve_step(const Raw<T> (&k1)[U], const Raw<T> (&k2)[U],
   }
 }
 
-// The serving form: one pass with running maxima and sums, each slot its own edges. Rows of k and v as
-// they come (any alignment, d and dv of 8 or more): packing every node's for a few rows would be most
-// of the call (70 000 nodes, 8 heads of d = 61, dv = 121 in bf16: about 110 us, the call itself 9 us for
-// 30 edges and 61 us for 65 537). The last chunk of a row then starts early enough to end with it; what it shares
-// with the chunk before is left out of q and k, and stored twice alike of the values.
+// The serving form: one pass with running maxima and sums, each slot its own edges. Rows of k and v
+// as they come (any alignment, d and dv of 8 or more): packing every node's for a few rows would be
+// most of the call (70 000 nodes, 8 heads of d = 61, dv = 121 in bf16: about 110 us, the call itself
+// 9 us for 30 edges and 61 us for 65 537). The last chunk of a row then starts early enough to end
+// with it; what it shares with the chunk before is left out of q and k, and stored twice alike of
+// the values.
 template <typename T, int G, int NV, bool BIAS>
 __global__ void __launch_bounds__(256) diff_serve_kernel(AttnArgs a) {
   constexpr int U = sizeof(T) == 4 ? 2 : 4;
