@@ -1757,8 +1757,11 @@ extern "C" int gatx_diff_attention_backward(
   GATX_REQUIRE(chunked(dtype, q, ldq) && chunked(dtype, k, ldk) && chunked(dtype, v, ldv) &&
                chunked(dtype, go, ldgo),
                "diff_attention_backward: rows of q, k, v, go must be 16-byte aligned (pack them)");
-  GATX_REQUIRE(hub_edges == 0 || (hubs && hub_count && (!by_source || (src_hubs && src_hub_count))),
-               "diff_attention_backward: null hub plan");
+  // each direction with its plan or without (NULL: it has no long rows, or walks them whole)
+  GATX_REQUIRE(hub_edges >= 0 && hub_bound >= 0 && src_hub_bound >= 0 && !hubs == !hub_count &&
+                   !src_hubs == !src_hub_count && (hubs || hub_bound == 0) &&
+                   (src_hubs || src_hub_bound == 0) && (hub_edges == 0 || hubs || src_hubs),
+               "diff_attention_backward: bad hub plan");
   const int dp = (int)round_up(d, 8), dvp = (int)round_up(dv, 8);
   const BackwardLayout l =
       backward_layout(N, E, heads, dp, dvp, gbias ? n_buckets : 0, hub_bound, src_hub_bound);

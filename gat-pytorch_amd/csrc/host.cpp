@@ -475,7 +475,11 @@ struct DiffAttentionBackward : public Node {
       out[3] = like(3, lt);
       if (bt.defined()) out[4] = like(4, bt);
       const int nb = out[4].defined() ? (int)bt.size(0) : 0;
-      const int64_t sb = srowptr.defined() ? src_hubs.bound : 0;
+      // either direction may be without a plan (no rows that long); both are of one length
+      const int pieces_of = hubs.edges ? hubs.edges : src_hubs.edges;
+      TORCH_CHECK(!src_hubs.edges || src_hubs.edges == pieces_of,
+                  "gatx: diff_attention: the plans of long rows differ in their pieces' length");
+      const int64_t sb = src_hubs.bound;
       const size_t wb = gatx_diff_attention_backward_workspace_bytes(csr.num_nodes, csr.edges, H, d,
                                                                      dv, nb, hubs.bound, sb);
       const Tensor ws = bytes(qt, wb), lp = packed(lt);
@@ -484,7 +488,7 @@ struct DiffAttentionBackward : public Node {
               ptr(rows[2].t), rows[2].ld, ptr(g.t), g.ld, H, d, dv, ints(csr.rowptr), ints(csr.col),
               ints(srowptr), ints(scol), ints(seid), csr.edges, csr.num_nodes, (float)scale,
               fptr(lp), (const uint8_t*)ptr(bucket), nb, fptr(S), fptr(stat), ptr(out[0]),
-              ptr(out[1]), ptr(out[2]), fptr(out[3]), fptr(out[4]), hubs.edges, ints(hubs.hubs),
+              ptr(out[1]), ptr(out[2]), fptr(out[3]), fptr(out[4]), pieces_of, ints(hubs.hubs),
               ints(hubs.count), hubs.bound, ints(src_hubs.hubs), ints(src_hubs.count), sb, ptr(ws),
               wb, ints(hubs.order), ints(src_hubs.order), stream_of(qt)),
           "diff_attention_backward");

@@ -669,8 +669,9 @@ int gatx_diff_attention(int dtype, const void* q, int64_t ldq, const void* k, in
                         size_t part_bytes, const int32_t* order, gatx_stream_t stream);
 /* Its gradients from go (num_nodes x (H,dvp), as v): gq, gk (num_nodes x (H,2,d)), gv
  * (num_nodes x (H,dv)), glam (H), gbias (n_buckets x H); each nullable. S and stat are the
- * forward's; srowptr / scol / seid the transposed CSR, with its own hub plan and order. Fixed-order
- * sums.
+ * forward's; srowptr / scol / seid the transposed CSR, with its own hub plan and order. Both plans are
+ * of hub_edges edges a piece; a direction whose hubs and count are NULL and whose bound is 0 has no
+ * plan and walks every row whole. Fixed-order sums.
  * workspace: gatx_diff_attention_backward_workspace_bytes(). */
 size_t gatx_diff_attention_backward_workspace_bytes(int64_t num_nodes, int64_t E, int num_heads,
                                                     int d, int dv, int n_buckets,
