@@ -78,25 +78,9 @@ def _needs(graph: Graph, built: bool, what: str):
                            "once eagerly)")
 
 
-def _ready(graph: Graph, key, built: bool):
-    """What the graph builds on first use may be used next on another stream: that one waits for
-    the build. (A capture begins after the device has caught up.)"""
-    if torch.cuda.is_current_stream_capturing():
-        return
-    now, done = stream(), graph._hub_plans.get((key, "built"))
-    if built:
-        event = torch.cuda.Event()
-        event.record()
-        graph._hub_plans[(key, "built")] = (now, event)
-    elif done is not None and done[0] != now:
-        torch.cuda.current_stream().wait_event(done[1])
-
-
 def _transpose(graph: Graph):
-    missing = graph.srowptr is None
-    _needs(graph, not missing, "transpose")
+    _needs(graph, graph.srowptr is not None, "transpose")
     graph.ensure_transpose()
-    _ready(graph, "transpose", missing)
     return graph.srowptr, graph.scol, graph.seid
 
 
@@ -110,17 +94,16 @@ def _row_order(graph: Graph, heads: int, source: bool):
     if graph.num_nodes * heads < _ORDER_ITEMS:
         return None
     key = ("order", source)
-    order = graph._hub_plans.get(key)
-    missing = order is None
-    if missing:
-        if graph._event is not None and torch.cuda.is_current_stream_capturing():
-            return None
+    if (key not in graph._hub_plans and graph._event is not None
+            and torch.cuda.is_current_stream_capturing()):
+        return None
+
+    def build():
         order = torch.empty((graph.num_nodes, 4), dtype=torch.int32, device=graph.device)
         call("gatx_diff_attention_row_order", ptr(graph.srowptr if source else graph.rowptr),
              graph.num_nodes, ptr(order), stream())
-        graph._hub_plans[key] = order
-    _ready(graph, key, missing)
-    return order
+        return (order,)
+    return graph.kept(key, build)[0]
 
 
 _NO_PLAN = (0, None, None, 0)
@@ -142,10 +125,8 @@ def _hub_plan(graph: Graph, source: bool):
     known = plans.get(key)
     if known == 0:
         return _NO_PLAN
-    missing = (T, source) not in plans
-    _needs(graph, not missing, "hub plan")
+    _needs(graph, (T, source) in plans, "hub plan")
     hubs, count, bound = graph.hub_plan(T, source)
-    _ready(graph, (T, source), missing)
     if not torch.cuda.is_current_stream_capturing():
         if known is None:
             # a graph built inside a capture has its counts only after a replay: never read

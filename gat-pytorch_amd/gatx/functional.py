@@ -1066,6 +1066,8 @@ def prepare_layer(x, edge_index, W, a, bias, num_heads, out_features, concat, ad
                            f"({num_heads * out_features}, {x.size(1)})")
     if graph is None:
         graph = graph_cache.get(edge_index, x.size(0), add_self_loops)
+    else:
+        graph.follow()
     # E' == 0 iff E == 0 (with the rewrite an empty edge_index already raised in Graph)
     if graph.num_input_edges == 0 and not const_attention:
         # attention_weights.max() of an empty tensor (models/gat_layer.py:85)

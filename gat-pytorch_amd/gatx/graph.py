@@ -19,6 +19,7 @@ at `Graph.poll()` (non-blocking, called by every layer on a cached graph) or at
 """
 from __future__ import annotations
 
+import threading
 import weakref
 from collections import OrderedDict
 
@@ -28,6 +29,14 @@ from . import _lib
 from ._lib import call, ptr, stream, version
 
 _I32_LIMIT = 2 ** 31 - 2
+
+# one thread builds what a Graph keeps at a time
+_BUILDING = threading.RLock()
+
+
+def _here(device) -> int:
+    """`device`'s current stream."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def _status_error(meta, N):
@@ -44,7 +53,10 @@ class Graph:
 
     rowptr [N+1], col [Eb] (source), rowidx [Eb] (destination), perm [Eb] (CSR slot -> position
     in edge_index'); srowptr / scol / seid: the source-ordered transpose, built on first use.
-    Eb = `edge_bound` >= E' is the allocation; kernels read E' from `e2_ptr` (device)."""
+    Eb = `edge_bound` >= E' is the allocation; kernels read E' from `e2_ptr` (device).
+
+    One Graph may be used on any stream: what it holds was filled on the stream that first needed
+    it, and another one waits for that before its first use (follow)."""
 
     def __init__(self, edge_index: torch.Tensor, num_nodes, add_self_loops: bool):
         """num_nodes None: size the node range from the edges (max id + 1; one host sync)."""
@@ -106,6 +118,7 @@ class Graph:
              ptr(self.perm), ptr(bws), ws_bytes, s)
         self.srowptr = self.scol = self.seid = None
         self._hub_plans = {}
+        self._builds = {}
         self._E2 = None
         # |edge_index'| promised by the caller (expect_num_edges): answers num_edges without a
         # device read (so a captured step may return edge_index' / alpha); checked against the
@@ -121,8 +134,53 @@ class Graph:
             self._meta_host.copy_(self.meta[:8], non_blocking=True)
             self._event = torch.cuda.Event()
             self._event.record()
+            self._built("csr", (self.meta, self.rowptr, self.col, self.rowidx, self.perm,
+                                self._ei_flat), self._event)
             check_pending(block=False)   # surfaces errors of earlier graphs that have landed
             _PENDING.append(weakref.ref(self))
+
+    # ---- streams
+    def _built(self, key, tensors, event=None, side=None):
+        """Tensors whose filling was just launched (on the current stream, or `side`), before anybody
+        else can find them. Nothing to keep inside a capture: replays are ordered by their caller."""
+        if event is None:
+            if torch.cuda.is_current_stream_capturing():
+                return
+            event = torch.cuda.Event()
+            event.record(*(() if side is None else (side,)))
+        # the stream itself is behind its launches (and behind a side stream once it has joined it)
+        self._builds[key] = (event, {_here(self.device)},
+                             [t for t in tensors if isinstance(t, torch.Tensor)])
+
+    def follow(self, key="csr"):
+        """The current stream behind the build of `key`, the memory kept for it. Inside a capture
+        nothing is waited for: the device has caught up when one begins."""
+        build = self._builds.get(key)
+        if build is None:
+            return
+        event, streams, tensors = build
+        here = _here(self.device)
+        if here in streams or torch.cuda.is_current_stream_capturing():
+            return
+        current = torch.cuda.current_stream(self.device)
+        current.wait_event(event)
+        for t in tensors:
+            t.record_stream(current)
+        streams.add(here)
+
+    def kept(self, key, build, side=None):
+        """What build() launched and returned (a tuple), once a graph and key."""
+        hit = self._hub_plans.get(key)
+        if hit is None:
+            with _BUILDING:
+                hit = self._hub_plans.get(key)
+                if hit is None:
+                    self.follow()
+                    hit = build()
+                    self._built(key, hit, side=side)
+                    self._hub_plans[key] = hit
+        self.follow(key)
+        return hit
 
     # ---- device-side sizes
     @property
@@ -152,9 +210,11 @@ class Graph:
             raise self._error
 
     def poll(self):
-        """Validate without blocking if the device has produced the meta (raises on bad ids)."""
+        """Validate without blocking if the device has produced the meta (raises on bad ids); the
+        current stream may use the CSR from here on."""
         if self._error is not None:
             raise self._error
+        self.follow()
         if (self._E2 is None and self._event is not None
                 and not torch.cuda.is_current_stream_capturing() and self._event.query()):
             self._validate(self._meta_host)
@@ -194,25 +254,32 @@ class Graph:
         return self._edge_index
 
     def ensure_transpose(self):
-        if self.srowptr is not None:
-            return
+        if self.srowptr is None:
+            with _BUILDING:
+                if self.srowptr is None:
+                    self._build_transpose()
+        self.follow("transpose")
+
+    def _build_transpose(self):
+        self.follow()
         N, Eb, dev = self.num_nodes, self.edge_bound, self.device
         i32 = dict(dtype=torch.int32, device=dev)
-        self.srowptr = torch.empty(N + 1, **i32)
-        self.scol = torch.empty(max(Eb, 1), **i32)
-        self.seid = torch.empty(max(Eb, 1), **i32)
+        srowptr = torch.empty(N + 1, **i32)
+        scol = torch.empty(max(Eb, 1), **i32)
+        seid = torch.empty(max(Eb, 1), **i32)
         ws_bytes = _lib.lib.gatx_graph_transpose_workspace_bytes(Eb, N)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
         call("gatx_graph_transpose", ptr(self.col), ptr(self.rowidx), N, Eb, self.e2_ptr,
-             ptr(self.srowptr), ptr(self.scol), ptr(self.seid), ptr(ws), ws_bytes, stream())
+             ptr(srowptr), ptr(scol), ptr(seid), ptr(ws), ws_bytes, stream())
+        self._built("transpose", (srowptr, scol, seid))
+        self.scol, self.seid = scol, seid
+        self.srowptr = srowptr   # the last: what others look at
 
     def hub_plan(self, hub_edges: int, source: bool = False):
         """(hubs, hub_count, hub_bound) of gatx_graph_hub_plan for this CSR: destination segments
         (source=True: source segments of the transpose, for the backward's source pass) longer
         than hub_edges listed as pieces (device-side count; built once per graph)."""
-        key = (hub_edges, source)
-        plan = self._hub_plans.get(key)
-        if plan is None:
+        def build():
             if source:
                 self.ensure_transpose()
             bound = int(_lib.lib.gatx_graph_hub_bound(self.edge_bound, hub_edges))
@@ -220,8 +287,8 @@ class Graph:
             count = torch.empty(1, dtype=torch.int32, device=self.device)
             call("gatx_graph_hub_plan", ptr(self.srowptr if source else self.rowptr),
                  self.num_nodes, hub_edges, ptr(hubs), bound, ptr(count), stream())
-            plan = self._hub_plans[key] = (hubs, count, bound)
-        return plan
+            return hubs, count, bound
+        return self.kept((hub_edges, source), build)
 
     def node_blocks(self, max_rows: int, side: bool = False):
         """(segs, count) of gatx_graph_segments for this CSR (device tensors, built once per graph
@@ -233,18 +300,17 @@ class Graph:
         joins it with join_side before reading the result), so the four small launches run
         under the projection GEMM instead of after it. The tensors are allocated on the current
         stream either way."""
-        key = ("blocks", max_rows)
-        hit = self._hub_plans.get(key)
-        if hit is None:
-            dev = self.device
+        from . import tuning
+        dev = self.device
+        sst = side_stream(dev) if side and tuning.get("side_stream") else None
+
+        def build():
             segs = torch.empty(_lib.lib.gatx_graph_segments_max() + 2, dtype=torch.int32,
                                device=dev)
             count = torch.empty(1, dtype=torch.int32, device=dev)
             wb = _lib.lib.gatx_graph_segments_workspace_bytes(self.num_nodes)
             ws = _seg_ws(dev, wb)
-            from . import tuning
-            if side and tuning.get("side_stream"):
-                sst = side_stream(dev)
+            if sst is not None:
                 sst.wait_stream(torch.cuda.current_stream(dev))
                 call("gatx_graph_segments", ptr(self.rowptr), ptr(self.col), self.num_nodes,
                      int(max_rows), ptr(segs), ptr(count), ptr(ws), wb, sst.cuda_stream)
@@ -253,8 +319,8 @@ class Graph:
                 join_side(dev)   # (the scratch may still be in use by a side-stream build)
                 call("gatx_graph_segments", ptr(self.rowptr), ptr(self.col), self.num_nodes,
                      int(max_rows), ptr(segs), ptr(count), ptr(ws), wb, stream())
-            hit = self._hub_plans[key] = (segs, count)
-        return hit
+            return segs, count
+        return self.kept(("blocks", max_rows), build, sst)
 
     def lds_blocks(self, max_rows: int, side: bool = False):
         """(segs, count, n_blocks) of node_blocks(max_rows) when this edge_index is known to cut
@@ -445,10 +511,12 @@ class GraphCache:
             ei = g._edge_index
             if (ei is not None and self._same(ei, edge_index)) or (
                     is_alias and self._same(t, edge_index)):
+                g.follow()
                 return g
         k = self._key(edge_index, -1, False)
         hit = self._d.get(k)
         if hit is not None:
+            hit[1].follow()
             return hit[1]
         g = Graph(edge_index, None, False)
         self._put(k, edge_index, g)
