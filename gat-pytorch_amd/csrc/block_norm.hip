@@ -4,10 +4,10 @@
 // and its gradients. With hn = h rh, yn = y ry, c = scale sigmoid(gate) weight:
 //   u   = gn next_weight;   g = gy + ry (u - yn mean(u yn))         (the gradient of y)
 //   gresid = g;  t = g c;   gh = rh (t - hn mean(t hn))
-//   ggate = g c hn (1 - sigmoid(gate))
+//   ggate = g c hn sigmoid(-gate)                    (1 - sigmoid(gate) would cancel where a gate is open)
 // The parameters' gradients are column sums of two products only: A = sum g sigmoid(gate) hn and
 // B = sum gn yn give gweight = scale A, gscale = weight A, gnext = B and, for a gate that is a
-// parameter, ggate = scale weight (1 - sigmoid(gate)) A.
+// parameter, ggate = scale weight sigmoid(-gate) A.
 //
 // HBM-bound: every input is read once and every output written once, a row's values stay in
 // registers between the two norms (y is not rounded on the way to the second one). One group of
@@ -16,7 +16,7 @@
 // backward's workgroups walk the rows in a fixed stride and keep A and B in registers; their
 // partial sums are added in workgroup order by a second launch.
 //
-// 44 900 x 1024 bf16, every part there: forward 82 us (460 MB, 5.6 TB/s), backward 192 (736 MB, 3.8
+// 44 900 x 1024 bf16, every part there: forward 82 us (460 MB, 5.6 TB/s), backward 199 (736 MB, 3.7
 // TB/s: the loads of a row wait for its two sums), column sums 5.
 #include "dtypes.h"
 
@@ -25,7 +25,7 @@ namespace {
 
 constexpr int kMaxCols = 8192;
 // Workgroups of the backward (their column partials): 3 a CU are what the registers of 16 elements of
-// five streams leave. 44 900 x 1024 bf16: 194 us with 768, 254 with 512, 255 with 1024 (a second
+// five streams leave. 44 900 x 1024 bf16 (one sigmoid an element): 194 us with 768, 254 with 512, 255 with 1024 (a second
 // round for a quarter of them), 200 with 1536; 128 registers (4 a CU) spill: 344 us; the next row's
 // loads in flight as well, or keeping a row unwidened between its two sums, cost the waves they need:
 // 262 and 277 us. A copy of the same bytes takes 144 us.
@@ -144,6 +144,18 @@ __global__ void __launch_bounds__(BLOCK ? 1024 : 256) norm_forward_kernel(NormAr
   }
 }
 
+// sigmoid(gate) and sigmoid(-gate) in one number: the smaller of them, whose difference from 1 is the
+// other to its last bit, with the sign set where that is sigmoid(-gate). The gradient of a gate needs
+// both, and 1 - sigmoid(gate) is nothing but rounding where a gate is open. (44 900 x 1024 bf16: 199
+// us; 195 with that difference; 212 with the gate loaded again for sigmoid(-gate).)
+__device__ inline float both_parts(float gate) {
+  const float t = __expf(-fabsf(gate));
+  return copysignf(t / (1.f + t), -gate);
+}
+__device__ inline bool is_open(float s) { return __float_as_int(s) < 0; }
+__device__ inline float open_part(float s) { return s + (is_open(s) ? 1.f : 0.f); }
+__device__ inline float shut_part(float s) { return (is_open(s) ? 0.f : 1.f) - s; }
+
 template <typename T, int VEC, int CH, bool BLOCK>
 __global__ void __launch_bounds__(BLOCK ? 1024 : 256) norm_backward_kernel(NormArgs a) {
   __shared__ float red[16];
@@ -164,7 +176,7 @@ __global__ void __launch_bounds__(BLOCK ? 1024 : 256) norm_backward_kernel(NormA
     const int64_t r = r0 + grp;
     const bool live = r < a.rows;
     const int64_t rr = live ? r : 0;
-    // hn, sigmoid(gate) and y; g starts as gy
+    // hn, the gate's factors and y; g starts as gy
     float hn[CH][VEC], sg[CH][VEC], y[CH][VEC], g[CH][VEC], gn[CH][VEC];
     const float rh = a.weight ? a.rstd_h[rr] : 1.f;
     const float ry = a.gn ? a.rstd_y[rr] : 0.f;
@@ -173,7 +185,7 @@ __global__ void __launch_bounds__(BLOCK ? 1024 : 256) norm_backward_kernel(NormA
     for (int c = 0; c < CH; ++c) {
       const int col = (c * lanes + li) * VEC;
       fill(hn[c], 0.f);
-      fill(sg[c], 1.f);
+      fill(sg[c], -0.f);   // no gate: open
       fill(g[c], 0.f);
       fill(gn[c], 0.f);
       fill(y[c], 0.f);
@@ -185,7 +197,7 @@ __global__ void __launch_bounds__(BLOCK ? 1024 : 256) norm_backward_kernel(NormA
         if (a.gate_rows) load_f32((const T*)a.gate + rr * a.ldg + col, sg[c]);
         else load_f32((const float*)a.gate + col, sg[c]);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) sg[c][i] = sigmoid(sg[c][i]);
+        for (int i = 0; i < VEC; ++i) sg[c][i] = both_parts(sg[c][i]);
       }
       if (a.gy) load_f32((const T*)a.gy + rr * a.ldgy + col, g[c]);
       if (a.gn) {
@@ -196,7 +208,7 @@ __global__ void __launch_bounds__(BLOCK ? 1024 : 256) norm_backward_kernel(NormA
         if (a.weight) {
           load_f32(a.weight + col, w);
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) y[c][i] *= w[i] * sg[c][i];
+          for (int i = 0; i < VEC; ++i) y[c][i] *= w[i] * open_part(sg[c][i]);
           if (a.scale) {
             load_f32(a.scale + col, w);
 #pragma unroll
@@ -248,12 +260,12 @@ __global__ void __launch_bounds__(BLOCK ? 1024 : 256) norm_backward_kernel(NormA
       }
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
-        const float gs = g[c][i] * sg[c][i];
+        const float gs = g[c][i] * open_part(sg[c][i]);
         if (live) A[c][i] = fmaf(gs, hn[c][i], A[c][i]);
         g[c][i] = gs * w[i];   // t
         x[i] = g[c][i] * hn[c][i];
         dot += x[i];
-        x[i] *= 1.f - sg[c][i];
+        x[i] *= shut_part(sg[c][i]);
       }
       if (live && a.ggate && a.gate_rows) store_f32((T*)a.ggate + r * a.cols + col, x);
     }
@@ -328,7 +340,7 @@ __global__ void __launch_bounds__(1024) norm_columns_kernel(NormArgs a, int part
   if (gweight) gweight[col] = sc * s;
   if (gscale) gscale[col] = w * s;
   if (a.ggate && !a.gate_rows)
-    ((float*)a.ggate)[col] = sc * w * (1.f - sigmoid(((const float*)a.gate)[col])) * s;
+    ((float*)a.ggate)[col] = sc * w * sigmoid(-((const float*)a.gate)[col]) * s;
 }
 
 // How a row is dealt out: `lanes` lanes with `ch` chunks each; lanes > 64: a workgroup.
