@@ -48,3 +48,23 @@ def test_gates_past_every_exponential(gate, device):
     for n, x in got.items():
         assert torch.isfinite(x).all(), n
     assert got["gate"].abs().max() < 1e-36
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_one_row_with_a_parameters_gate(dtype, device):
+    """h (D,) and a float32 gate (D,): what the same row gives as a batch of one, bit by bit."""
+    from gatx import BlockNorm
+    m = BlockNorm(40).to(device)
+    g = torch.Generator().manual_seed(3)
+    with torch.no_grad():
+        for p in m.parameters():
+            p.copy_(torch.randn(40, generator=g))
+    h, r, gy, gn = (torch.randn(40, generator=g).to(dtype).to(device) for _ in range(4))
+
+    def step(h, r, gy, gn):
+        x = [h.clone().requires_grad_(True), r.clone().requires_grad_(True)]
+        outs = m(x[0], x[1])
+        return [o.detach().flatten() for o in outs] + [
+            y.flatten() for y in torch.autograd.grad(outs, x + list(m.parameters()), [gy, gn])]
+    one, batch = step(h, r, gy, gn), step(h[None], r[None], gy[None], gn[None])
+    assert all(torch.equal(a, b) for a, b in zip(one, batch))
