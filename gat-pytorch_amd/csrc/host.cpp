@@ -231,9 +231,7 @@ Tensor norm_before(const Tensor& x, const Tensor& weight, double eps) {
 py::object norm_after(const Tensor& h, const Tensor& weight, const Opt& resid_, const Opt& gate_,
                       const Opt& scale_, const Opt& next_weight_, double eps) {
   const Tensor resid = of(resid_), gate = of(gate_), scale = of(scale_), next_weight = of(next_weight_);
-  // of one row (1-D) a gate of another type is the parameter; of its own both readings are one
-  const bool gate_rows = gate.defined() && !(gate.dim() == 1 && (h.dim() != 1 ||
-                                             gate.scalar_type() != h.scalar_type()));
+  const bool gate_rows = gate.defined() && gate.dim() != 1;   // (one row's gate is a parameter's)
   check_norm("norm_after", h,
              {{"weight", weight}, {"scale", scale}, {"next_weight", next_weight},
               {"gate", gate_rows ? Tensor() : gate}},
