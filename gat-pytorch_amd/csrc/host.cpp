@@ -13,6 +13,8 @@
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
 
+#include <unordered_set>
+
 #include "../../include/gatx.h"
 
 namespace {
@@ -65,16 +67,28 @@ void no_tangents(const char* what, const In&... inputs) {
 
 // A captured backward into a leaf that an eager graph on the default stream still holds would make
 // that stream, which cannot take part in a capture, wait for the captured one: the capture breaks
-// on the engine's thread, where nothing can be caught.
-void check_capture(const Node& node, const char* what) {
+// on the engine's thread, where nothing can be caught, and the process ends. So it is looked for before
+// the first launch, over everything this backward goes on to (a leaf can be behind the cast of a 16-bit
+// parameter, a view, any operation); leaves whose gradients nobody asks for do not count.
+void check_capture(Node& node, const char* what) {
   if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
-  for (const auto& edge : node.next_edges()) {
-    if (!edge.function || edge.function->num_outputs() != 0) continue;
-    const auto stream = edge.function->stream();
-    TORCH_CHECK(!stream || stream->id() != 0, "gatx: ", what,   // (0: the default stream)
-                ": the captured backward reaches a leaf of an autograd graph that is alive on the "
-                "default stream; drop that graph's results, or run the eager steps on the capture's "
-                "stream");
+  std::vector<Node*> todo = {&node};
+  std::unordered_set<Node*> seen = {&node};
+  while (!todo.empty()) {
+    Node* at = todo.back();
+    todo.pop_back();
+    for (size_t i = 0; i < at->num_outputs(); ++i) {
+      if (!at->task_should_compute_output(i)) continue;
+      Node* next = at->next_edge(i).function.get();
+      if (!next || !seen.insert(next).second) continue;
+      todo.push_back(next);
+      if (next->num_outputs() != 0) continue;
+      const auto stream = next->stream();
+      TORCH_CHECK(!stream || stream->id() != 0, "gatx: ", what,   // (0: the default stream)
+                  ": the captured backward reaches a leaf of an autograd graph that is alive on the "
+                  "default stream; drop that graph's results, or run the eager steps on the capture's "
+                  "stream");
+    }
   }
 }
 
