@@ -26,7 +26,7 @@ from collections import OrderedDict
 import torch
 
 from . import _lib
-from ._lib import call, ptr, stream, version
+from ._lib import call, on_device, ptr, stream, version
 
 _I32_LIMIT = 2 ** 31 - 2
 
@@ -56,7 +56,8 @@ class Graph:
     Eb = `edge_bound` >= E' is the allocation; kernels read E' from `e2_ptr` (device).
 
     One Graph may be used on any stream: what it holds was filled on the stream that first needed
-    it, and another one waits for that before its first use (follow)."""
+    it, and another one waits for that before its first use (follow). It is built on its edges'
+    device, whichever is current."""
 
     def __init__(self, edge_index: torch.Tensor, num_nodes, add_self_loops: bool):
         """num_nodes None: size the node range from the edges (max id + 1; one host sync)."""
@@ -66,10 +67,14 @@ class Graph:
             raise RuntimeError(f"edge_index must be int64 or int32, got {edge_index.dtype}")
         if not edge_index.is_cuda:
             raise RuntimeError("gatx: edge_index must be on the HIP device (no CPU path)")
-        dev = edge_index.device
+        self.device = edge_index.device
+        with on_device(self.device):
+            self._build_csr(edge_index, num_nodes, add_self_loops)
+
+    def _build_csr(self, edge_index, num_nodes, add_self_loops):
+        dev = self.device
         if edge_index.stride(1) != 1:
             edge_index = edge_index.contiguous()
-        self.device = dev
         self.add_self_loops = add_self_loops
         self.source = edge_index
         E = edge_index.size(1)
@@ -160,19 +165,22 @@ class Graph:
             return
         event, streams, tensors = build
         here = _here(self.device)
-        if here in streams or torch.cuda.is_current_stream_capturing():
+        if here in streams:
             return
-        current = torch.cuda.current_stream(self.device)
-        current.wait_event(event)
-        for t in tensors:
-            t.record_stream(current)
+        with on_device(self.device):
+            if torch.cuda.is_current_stream_capturing():
+                return
+            current = torch.cuda.current_stream()
+            current.wait_event(event)
+            for t in tensors:
+                t.record_stream(current)
         streams.add(here)
 
     def kept(self, key, build, side=None):
         """What build() launched and returned (a tuple), once a graph and key."""
         hit = self._hub_plans.get(key)
         if hit is None:
-            with _BUILDING:
+            with _BUILDING, on_device(self.device):
                 hit = self._hub_plans.get(key)
                 if hit is None:
                     self.follow()
@@ -255,7 +263,7 @@ class Graph:
 
     def ensure_transpose(self):
         if self.srowptr is None:
-            with _BUILDING:
+            with _BUILDING, on_device(self.device):
                 if self.srowptr is None:
                     self._build_transpose()
         self.follow("transpose")

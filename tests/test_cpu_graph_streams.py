@@ -190,3 +190,52 @@ def test_nobody_finds_what_has_no_event_yet(rec, monkeypatch):
     for t in threads:
         t.join()
     assert launches(rec) == ["gatx_graph_hub_plan"]
+
+
+class OnDevice(torch.Tensor):
+    """A host tensor that says it is on the device."""
+    is_cuda = True
+
+
+@pytest.mark.parametrize("what", ["csr", "order"] + list(USES))
+def test_everything_is_launched_on_the_graphs_own_device(what, rec, monkeypatch):
+    """... whichever is current."""
+    import contextlib
+
+    from gatx import attention, graph
+    inside = []
+
+    @contextlib.contextmanager
+    def on_device(device):
+        inside.append(device)
+        yield
+        inside.pop()
+    seen = []
+    for module in (graph, attention):
+        monkeypatch.setattr(module, "on_device", on_device)
+        monkeypatch.setattr(module, "call", lambda name, *a: seen.append((name, list(inside))))
+    monkeypatch.setattr(graph, "_seg_ws", lambda dev, n: torch.zeros(1))
+    monkeypatch.setattr(graph, "_META_WS", {})
+    monkeypatch.setattr(graph, "_PENDING", [])
+    empty = torch.empty
+    monkeypatch.setattr(torch, "empty", lambda *a, pin_memory=False, **k: empty(*a, **k))
+    event, record = torch.cuda.Event, []
+
+    class Event(event):
+        def record(self, stream=None):
+            record.append(list(inside))
+            super().record(stream)
+    if what == "csr":
+        monkeypatch.setattr(torch.cuda, "Event", Event)
+        graph.Graph(torch.zeros(2, 9, dtype=torch.int64).as_subclass(OnDevice), 5, True)
+    else:
+        g = built(rec)
+        monkeypatch.setattr(torch.cuda, "Event", Event)
+        if what == "order":
+            monkeypatch.setattr(attention, "_ORDER_ITEMS", 1)
+            attention._row_order(g, 2, False)
+        else:
+            USES[what](g)
+    assert seen and all(x == torch.device("cpu") for _, d in seen for x in d)
+    assert all(d for _, d in seen), seen
+    assert record and all(record)
