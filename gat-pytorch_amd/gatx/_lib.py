@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 import os
 
 import torch  # noqa: F401  (must precede the CDLL: shares torch's libamdhip64)
@@ -236,6 +237,22 @@ def on_device(device):
     if device.index is None or device.index == torch._C._cuda_getDevice():
         return _HERE_CTX
     return torch.cuda.device(device)
+
+
+def untraced(fn):
+    """fn, which torch.compile calls and does not look into: it may use streams and events. (Traced, they
+    become weak references of the compiler's, which it still follows after their owner is gone: the
+    process ends.) Outside of a trace it costs a flag's test, and imports nothing."""
+    opaque = []
+
+    @functools.wraps(fn)
+    def either(*args, **kwargs):
+        if torch.compiler.is_compiling():
+            if not opaque:
+                opaque.append(torch.compiler.disable(fn))
+            return opaque[0](*args, **kwargs)
+        return fn(*args, **kwargs)
+    return either
 
 
 def call(name: str, *args):

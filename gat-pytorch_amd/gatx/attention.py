@@ -16,7 +16,7 @@ import torch
 from torch import nn
 
 from . import tuning
-from ._lib import DTYPES, call, host as _host, on_device, ptr, stream
+from ._lib import DTYPES, call, host as _host, on_device, ptr, stream, untraced
 from .graph import Graph, graph_cache
 
 MAX_HEAD_WIDTH = 256    # d
@@ -80,7 +80,7 @@ def _needs(graph: Graph, built: bool, what: str):
 
 def _transpose(graph: Graph):
     _needs(graph, graph.srowptr is not None, "transpose")
-    graph.ensure_transpose()
+    graph._ensure_transpose()
     return graph.srowptr, graph.scol, graph.seid
 
 
@@ -103,7 +103,7 @@ def _row_order(graph: Graph, heads: int, source: bool):
         call("gatx_diff_attention_row_order", ptr(graph.srowptr if source else graph.rowptr),
              graph.num_nodes, ptr(order), stream())
         return (order,)
-    return graph.kept(key, build)[0]
+    return graph._kept(key, build)[0]
 
 
 _NO_PLAN = (0, None, None, 0)
@@ -183,6 +183,7 @@ def _check(q, k, v, lam, graph, bias, positions, nodes):
         raise ValueError("gatx: diff_attention: nodes is a 1-D int32 or int64 tensor")
 
 
+@untraced
 def diff_attention(q, k, v, lam, graph: Graph, *, scale=None, bias=None, positions=None,
                    max_distance: int = 128, bidirectional: bool = True, nodes=None):
     """Differential attention of every node over its in-neighbours in `graph`.
@@ -205,7 +206,7 @@ def diff_attention(q, k, v, lam, graph: Graph, *, scale=None, bias=None, positio
 
     Gradients: q, k, v, lam, bias, once differentiable, the same bits every time."""
     _check(q, k, v, lam, graph, bias, positions, nodes)
-    graph.poll()
+    graph._poll()
     scale = 1.0 / math.sqrt(q.size(3)) if scale is None else float(scale)
     exact, bounds = (0, []) if bias is None else _bounds(bias.size(0), int(max_distance),
                                                          bool(bidirectional))

@@ -26,7 +26,7 @@ from collections import OrderedDict
 import torch
 
 from . import _lib
-from ._lib import call, on_device, ptr, stream, version
+from ._lib import call, on_device, ptr, stream, untraced, version
 
 _I32_LIMIT = 2 ** 31 - 2
 
@@ -59,6 +59,7 @@ class Graph:
     it, and another one waits for that before its first use (follow). It is built on its edges'
     device, whichever is current."""
 
+    @untraced
     def __init__(self, edge_index: torch.Tensor, num_nodes, add_self_loops: bool):
         """num_nodes None: size the node range from the edges (max id + 1; one host sync)."""
         if edge_index.dim() != 2 or edge_index.size(0) != 2:
@@ -176,7 +177,7 @@ class Graph:
                 t.record_stream(current)
         streams.add(here)
 
-    def kept(self, key, build, side=None):
+    def _kept(self, key, build, side=None):
         """What build() launched and returned (a tuple), once a graph and key."""
         hit = self._hub_plans.get(key)
         if hit is None:
@@ -217,7 +218,7 @@ class Graph:
                 f"{self._E2_hint} for this edge_index (its contents changed?)")
             raise self._error
 
-    def poll(self):
+    def _poll(self):
         """Validate without blocking if the device has produced the meta (raises on bad ids); the
         current stream may use the CSR from here on."""
         if self._error is not None:
@@ -226,6 +227,8 @@ class Graph:
         if (self._E2 is None and self._event is not None
                 and not torch.cuda.is_current_stream_capturing() and self._event.query()):
             self._validate(self._meta_host)
+
+    poll = untraced(_poll)
 
     # ---- host-side sizes (synchronise on first use)
     @property
@@ -241,6 +244,7 @@ class Graph:
             self._read_meta()
         return self._E2
 
+    @untraced
     def _read_meta(self):
         if self._event is not None:
             self._event.synchronize()
@@ -261,12 +265,14 @@ class Graph:
                 graph_cache.alias(self._edge_index, self)
         return self._edge_index
 
-    def ensure_transpose(self):
+    def _ensure_transpose(self):
         if self.srowptr is None:
             with _BUILDING, on_device(self.device):
                 if self.srowptr is None:
                     self._build_transpose()
         self.follow("transpose")
+
+    ensure_transpose = untraced(_ensure_transpose)
 
     def _build_transpose(self):
         self.follow()
@@ -283,21 +289,23 @@ class Graph:
         self.scol, self.seid = scol, seid
         self.srowptr = srowptr   # the last: what others look at
 
+    @untraced
     def hub_plan(self, hub_edges: int, source: bool = False):
         """(hubs, hub_count, hub_bound) of gatx_graph_hub_plan for this CSR: destination segments
         (source=True: source segments of the transpose, for the backward's source pass) longer
         than hub_edges listed as pieces (device-side count; built once per graph)."""
         def build():
             if source:
-                self.ensure_transpose()
+                self._ensure_transpose()
             bound = int(_lib.lib.gatx_graph_hub_bound(self.edge_bound, hub_edges))
             hubs = torch.empty((max(bound, 1), 4), dtype=torch.int32, device=self.device)
             count = torch.empty(1, dtype=torch.int32, device=self.device)
             call("gatx_graph_hub_plan", ptr(self.srowptr if source else self.rowptr),
                  self.num_nodes, hub_edges, ptr(hubs), bound, ptr(count), stream())
             return hubs, count, bound
-        return self.kept((hub_edges, source), build)
+        return self._kept((hub_edges, source), build)
 
+    @untraced
     def node_blocks(self, max_rows: int, side: bool = False):
         """(segs, count) of gatx_graph_segments for this CSR (device tensors, built once per graph
         and max_rows): contiguous node blocks no edge crosses, each <= max_rows nodes; count -1
@@ -328,7 +336,7 @@ class Graph:
                 call("gatx_graph_segments", ptr(self.rowptr), ptr(self.col), self.num_nodes,
                      int(max_rows), ptr(segs), ptr(count), ptr(ws), wb, stream())
             return segs, count
-        return self.kept(("blocks", max_rows), build, sst)
+        return self._kept(("blocks", max_rows), build, sst)
 
     def lds_blocks(self, max_rows: int, side: bool = False):
         """(segs, count, n_blocks) of node_blocks(max_rows) when this edge_index is known to cut
@@ -486,13 +494,14 @@ class GraphCache:
         return (t.data_ptr(), version(t), tuple(t.shape), tuple(t.stride()), t.dtype,
                 t.device, num_nodes, add_self_loops)
 
+    @untraced
     def get(self, edge_index: torch.Tensor, num_nodes: int, add_self_loops: bool) -> Graph:
         k = self._key(edge_index, num_nodes, add_self_loops)
         hit = self._d.get(k)
         if hit is not None:
             self._d.move_to_end(k)
             g = hit[1]
-            g.poll()
+            g._poll()
             return g
         g = Graph(edge_index, num_nodes, add_self_loops)
         self._put(k, edge_index, g)
@@ -511,6 +520,7 @@ class GraphCache:
                           and a.shape == b.shape and a.stride() == b.stride()
                           and a.dtype == b.dtype and a.device == b.device)
 
+    @untraced
     def for_edges(self, edge_index: torch.Tensor) -> Graph:
         """The Graph whose edge_index' IS this tensor (what a layer returned), else a CSR of it
         as given (no rewrite), sized by its max id — for consumers of a layer's output edges
