@@ -89,8 +89,8 @@ _ORDER_ITEMS = 8192
 
 
 def _row_order(graph: Graph, heads: int, source: bool):
-    """The rows by length (csrc/diff_attn.hip, row_order_kernel), for rows that share waves. No result
-    depends on it, so a capture that finds none goes without."""
+    """The rows by length (csrc/diff_attn.hip, row_order_kernel), for rows that share waves. No
+    result depends on it, so a capture that finds none goes without."""
     if graph.num_nodes * heads < _ORDER_ITEMS:
         return None
     key = ("order", source)

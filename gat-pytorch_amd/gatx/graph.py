@@ -90,7 +90,7 @@ class Graph:
         # {E2, num_loops, status, min, max, self-loops, nb, chunk} + the compaction's block
         # offsets (GATX_META_WORDS); the host only ever reads the first 8
         self.meta = torch.empty(_lib.META_WORDS, dtype=torch.int64, device=dev)
-        ws = _meta_ws(dev)
+        ws = torch.empty(_lib.lib.gatx_graph_meta_workspace_bytes(), dtype=torch.uint8, device=dev)
         if num_nodes is None:   # sized by the edges themselves: the one case that must sync
             call("gatx_graph_meta", ptr(edge_index), is64, E, ld, int(add_self_loops),
                  _I32_LIMIT, ptr(self.meta), ptr(ws), s)
@@ -147,8 +147,8 @@ class Graph:
 
     # ---- streams
     def _built(self, key, tensors, event=None, side=None):
-        """Tensors whose filling was just launched (on the current stream, or `side`), before anybody
-        else can find them. Nothing to keep inside a capture: replays are ordered by their caller."""
+        """Tensors whose filling was just launched (on the current stream, or `side`), before
+        anybody else can find them. Nothing to keep inside a capture: whoever replays it orders it."""
         if event is None:
             if torch.cuda.is_current_stream_capturing():
                 return
@@ -365,7 +365,6 @@ class Graph:
         return self.rowptr.cpu(), self.col[:E2].cpu(), self.perm[:E2].cpu()
 
 
-_META_WS = {}
 _PENDING: list = []
 _HINTS: dict = {}
 _BLOCKS: dict = {}   # edge_index identity -> node-block count (<= 0: no LDS-staged passes)
@@ -445,14 +444,6 @@ def _seg_ws(dev, nbytes: int):
         if t is not None:
             _SEG_WS_RETIRED.append(t)   # a captured graph may still launch on the old one
         t = _SEG_WS[dev] = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)
-    return t
-
-
-def _meta_ws(dev):
-    t = _META_WS.get(dev)
-    if t is None:
-        t = torch.empty(_lib.lib.gatx_graph_meta_workspace_bytes(), dtype=torch.uint8, device=dev)
-        _META_WS[dev] = t
     return t
 
 

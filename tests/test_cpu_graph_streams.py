@@ -215,7 +215,6 @@ def test_everything_is_launched_on_the_graphs_own_device(what, rec, monkeypatch)
         monkeypatch.setattr(module, "on_device", on_device)
         monkeypatch.setattr(module, "call", lambda name, *a: seen.append((name, list(inside))))
     monkeypatch.setattr(graph, "_seg_ws", lambda dev, n: torch.zeros(1))
-    monkeypatch.setattr(graph, "_META_WS", {})
     monkeypatch.setattr(graph, "_PENDING", [])
     empty = torch.empty
     monkeypatch.setattr(torch, "empty", lambda *a, pin_memory=False, **k: empty(*a, **k))
@@ -239,3 +238,23 @@ def test_everything_is_launched_on_the_graphs_own_device(what, rec, monkeypatch)
     assert seen and all(x == torch.device("cpu") for _, d in seen for x in d)
     assert all(d for _, d in seen), seen
     assert record and all(record)
+
+
+def test_graphs_built_at_once_share_no_workspace(rec, monkeypatch):
+    """On two streams (or one of them in a replayed capture): what one writes between its launches is its
+    own."""
+    from gatx import graph
+    alive, used = [], []
+    empty = torch.empty
+
+    def kept(*a, pin_memory=False, **k):
+        alive.append(empty(*a, **k))   # nothing's memory is handed out again
+        return alive[-1]
+    monkeypatch.setattr(torch, "empty", kept)
+    monkeypatch.setattr(graph, "_PENDING", [])
+    monkeypatch.setattr(graph, "call", lambda name, *a: used.append((name, a)))
+    for _ in range(2):
+        graph.Graph(torch.zeros(2, 9, dtype=torch.int64).as_subclass(OnDevice), 5, True)
+    meta = [a[7] for name, a in used if name == "gatx_graph_meta"]
+    build = [a[13] for name, a in used if name == "gatx_graph_build"]
+    assert len(set(meta)) == len(set(build)) == 2

@@ -67,6 +67,28 @@ def test_the_second_stream_waits(first, second, device):
         del junk
 
 
+def test_graphs_built_on_several_streams_at_once(device):
+    """Many small graphs, each with its own sizes, ids and self-loops, on four streams in turn."""
+    from gatx.graph import Graph
+    g = torch.Generator().manual_seed(5)
+    edges = [torch.randint(0, 50 + 37 * i, (2, 3000 + 711 * i), generator=g).to(device)
+             for i in range(12)]
+    for e in edges[::2]:
+        e[1, ::3] = e[0, ::3]   # self-loops, dropped
+    want = [Graph(e, int(e.max()) + 1, True).csr_host() for e in edges]
+    sizes = [int(e.max()) + 1 for e in edges]
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    for _ in range(5):
+        torch.cuda.synchronize()
+        built = []
+        for i, e in enumerate(edges):
+            with torch.cuda.stream(streams[i % 4]):
+                built.append(Graph(e, sizes[i], True))
+        torch.cuda.synchronize()
+        for got, w in zip(built, want):
+            assert all(torch.equal(a, b) for a, b in zip(got.csr_host(), w))
+
+
 def test_the_graph_cache_hands_a_graph_to_another_stream(device):
     """DiffAttention and GATLayer find the graph of an edge_index in the cache."""
     import gatx
